@@ -1,4 +1,4 @@
-"""ctypes bindings of include/flagcx_amd/fx_kernels.h and fx_synth.h."""
+"""ctypes bindings of include/flagcx_amd/fx_kernels.h, fx_model.h and fx_synth.h."""
 import ctypes as C
 import os
 
@@ -15,6 +15,7 @@ SUCCESS, DEVICE_ERROR, SYSTEM_ERROR, INTERNAL_ERROR, INVALID_ARGUMENT = 0, 1, 2,
 INVALID_USAGE, IN_PROGRESS, NOT_SUPPORTED = 5, 7, 9
 DT_INT8, DT_UINT8, DT_INT32, DT_UINT32, DT_INT64, DT_UINT64 = 0, 1, 2, 3, 4, 5
 DT_FP16, DT_FP32, DT_FP64, DT_BF16 = 6, 7, 8, 9
+DT_E4M3 = 0x40             # FX_E4M3 of include/flagcx_amd/fx_model.h: not a FlagCX datatype
 OP_SUM, OP_PROD, OP_MAX, OP_MIN, OP_AVG = 0, 1, 2, 3, 4
 MEMCPY_H2D, MEMCPY_D2H, MEMCPY_D2D = 0, 1, 2
 MEM_HOST, MEM_DEVICE, MEM_MANAGED = 0, 1, 2
@@ -172,6 +173,46 @@ _SIGS.update({
     "fx_part_ring_ar": (_sz, [_sz, _i, _i, _sz, _sz, C.POINTER(RedNode)]),
     "fx_part_ring_rs": (_sz, [_sz, _i, _i, _sz, _sz, C.POINTER(RedNode)]),
     "fx_part_locred": (_sz, [_sz, _i, _i, _sz, C.POINTER(RedNode)]),
+})
+
+
+class _Strides(C.Structure):
+    """Row strides in elements; the fields of a call's stride block in the header's order."""
+
+    @classmethod
+    def of(cls, strides):
+        """A dict with every field, or None (dense rows), as the pointer the C call takes."""
+        return None if strides is None else C.byref(cls(**strides))
+
+
+class NormStrides(_Strides):
+    _fields_ = [(f, _sz) for f in ("in_", "residual", "total", "out", "scale")]
+
+
+class NormGradStrides(_Strides):
+    _fields_ = [(f, _sz) for f in ("dy", "x", "dtotal", "dx")]
+
+
+class ProductStrides(_Strides):
+    _fields_ = [(f, _sz) for f in ("x", "w", "y", "expert_w")]
+
+
+class ProductDwStrides(_Strides):
+    _fields_ = [(f, _sz) for f in ("dy", "x", "dw", "expert_dw")]
+
+
+class ProductE4m3Strides(_Strides):
+    _fields_ = [(f, _sz) for f in ("x", "w", "y", "expert_w", "xscale", "wscale", "expert_wscale")]
+
+
+_SIGS.update({
+    # include/flagcx_amd/fx_model.h
+    "fx_reduce_norm": (_i, [_vp, _vp, _vp, C.POINTER(_vp), _i, _vp, _vp, _sz, _sz, _vp, _i, _i, _i, C.c_float, _vp]),
+    "fx_reduce_norm_grad_workspace": (_sz, [_sz, _sz]),
+    "fx_reduce_norm_grad": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _i, _i, C.c_float, _vp, _sz, _vp]),
+    "fx_expert_product": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _i, _vp, _i, _i, _vp]),
+    "fx_expert_product_dw": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _i, _i, _vp]),
+    "fx_expert_product_e4m3": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _i, _vp]),
 })
 for _name, (_res, _args) in _SIGS.items():
     _f = getattr(lib, _name)

@@ -1,0 +1,581 @@
+// k-way sum + residual + root-mean-square norm (fx_reduce_norm) and its gradients
+// (fx_reduce_norm_grad).
+//
+// A row of C columns is held in the registers of TPR threads, V octets each
+// (octet i * TPR + t belongs to thread t, so 16 neighbouring lanes hold one scale
+// group of 128 columns): inputs are read once, the row's sum of squares is
+// reduced over the threads, and the results leave from the same registers.  The
+// arithmetic is a few operations per element; HBM bounds it.  Rows longer than
+// kHeld columns are read twice (the second pass mostly from the caches).
+#include "flagcx_amd/fx_kernels.h"
+#include "flagcx_amd/fx_model.h"
+#include "fx_vec.hpp"
+
+using namespace fx;
+
+namespace {
+
+constexpr uint32_t kHeld = 1024 * 4 * 8;      // widest row held in registers: 1024 threads, 4 octets each
+constexpr float kE4m3Max = 448.f;
+constexpr float kTinyScale = 0x1p-126f;
+
+struct NormArgs {
+  const void *in[FX_MAX_INPUTS + 1];          // k inputs and the residual, if any, behind them
+  void *total, *out;
+  float *scale;
+  const void *weight;
+  size_t ldIn, ldRes, ldTotal, ldOut, ldScale;
+  uint32_t rows, cols, n;                     // n = entries of `in`
+  uint32_t k;
+  float eps;
+  uint32_t weightF32;
+};
+
+__device__ __forceinline__ float blockSum(float x, float *lds, uint32_t nWaves) {
+  x = waveSum(x);
+  if (nWaves == 1) return x;
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+  __syncthreads();
+  float s = 0.f;
+  for (uint32_t w = 0; w < nWaves; w++) s += lds[w];
+  __syncthreads();
+  return s;
+}
+
+// The octet's sum over all inputs, left to right.  B inputs are loaded before the
+// first is used.
+template <class T, int V, int B>
+__device__ __forceinline__ void sumInputs(const NormArgs &a, uint32_t row, const uint32_t (&c)[V], float (&f)[V][8]) {
+#pragma unroll
+  for (int i = 0; i < V; i++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) f[i][j] = 0.f;
+  for (uint32_t p0 = 0; p0 < a.n; p0 += B) {
+    Octet<T> v[B][V];
+#pragma unroll
+    for (int b = 0; b < B; b++)
+      if (p0 + b < a.n) {
+        const T *r = (const T *)a.in[p0 + b] + (size_t)row * (p0 + b < a.k ? a.ldIn : a.ldRes);
+#pragma unroll
+        for (int i = 0; i < V; i++) v[b][i] = loadOctet(r, c[i], a.cols);
+      }
+#pragma unroll
+    for (int b = 0; b < B; b++)
+      if (p0 + b < a.n) {
+        const bool first = p0 + b == 0;       // 0 + x would turn -0 into +0
+#pragma unroll
+        for (int i = 0; i < V; i++)
+#pragma unroll
+          for (int j = 0; j < 8; j++) f[i][j] = first ? v[b][i].get(j) : f[i][j] + v[b][i].get(j);
+      }
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void weights(const NormArgs &a, uint32_t c, float (&w)[8]) {
+  if (!a.weight) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) w[j] = 1.f;
+  } else if (sizeof(T) == 4 || a.weightF32) {
+    const Octet<float> o = loadOctet((const float *)a.weight, c, a.cols);
+#pragma unroll
+    for (int j = 0; j < 8; j++) w[j] = o.get(j);
+  } else {
+    const Octet<T> o = loadOctet((const T *)a.weight, c, a.cols);
+#pragma unroll
+    for (int j = 0; j < 8; j++) w[j] = o.get(j);
+  }
+}
+
+template <class T, bool QUANT>
+__device__ __forceinline__ void finishOctet(const NormArgs &a, uint32_t row, uint32_t c, const float (&f)[8], float r) {
+  float w[8], y[8];
+  weights<T>(a, c, w);
+#pragma unroll
+  for (int j = 0; j < 8; j++) y[j] = f[j] * r * w[j];
+  if (a.total) storeOctet((T *)a.total + (size_t)row * a.ldTotal, c, a.cols, f);
+  if constexpr (QUANT) {
+    // The largest magnitude as an integer: NaN > infinity > finite, so a NaN gets through.
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const uint32_t b = c + j < a.cols ? (__builtin_bit_cast(uint32_t, y[j]) & 0x7fffffffu) : 0u;
+      m = m > b ? m : b;
+    }
+#pragma unroll
+    for (int d = 8; d; d >>= 1) {
+      const uint32_t o = (uint32_t)__shfl_xor((int)m, d);
+      m = m > o ? m : o;
+    }
+    const float amax = __builtin_bit_cast(float, m);
+    float scale = amax / kE4m3Max;
+    scale = scale < kTinyScale ? kTinyScale : scale;          // NaN compares false and stays
+    const float inv = 1.f / scale;
+#pragma unroll
+    for (int j = 0; j < 8; j++) y[j] *= inv;
+    storeE4m3((uint8_t *)a.out + (size_t)row * a.ldOut, c, a.cols, y);
+    if ((threadIdx.x & 15) == 0 && c < a.cols) a.scale[(size_t)row * a.ldScale + c / FX_SCALE_GROUP] = scale;
+  } else {
+    storeOctet((T *)a.out + (size_t)row * a.ldOut, c, a.cols, y);
+  }
+}
+
+// One row per TPR threads; with TPR = 64 a workgroup of 256 takes four rows, one per wavefront.
+template <class T, int TPR, int V, bool QUANT>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) normRows(NormArgs a) {
+  constexpr uint32_t kPer = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float lds[16];
+  const uint32_t row = blockIdx.x * kPer + threadIdx.x / TPR;
+  if (row >= a.rows) return;                  // whole wavefronts leave; kPer > 1 has no barrier
+  uint32_t c[V];
+#pragma unroll
+  for (int i = 0; i < V; i++) c[i] = (i * TPR + threadIdx.x % TPR) * 8;
+  float f[V][8];
+  sumInputs<T, V, (V == 1 ? 8 : V == 2 ? 4 : 2)>(a, row, c, f);
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; i++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) q = __builtin_fmaf(f[i][j], f[i][j], q);
+  q = blockSum(q, lds, TPR / 64);
+  const float r = 1.f / sqrtf(q / (float)a.cols + a.eps);
+#pragma unroll
+  for (int i = 0; i < V; i++) finishOctet<T, QUANT>(a, row, c[i], f[i], r);
+}
+
+// Rows wider than the registers hold: the sum is formed twice.  Every element is
+// read and written by one thread in the second pass, so exact aliasing is safe.
+template <class T, bool QUANT>
+__global__ void __launch_bounds__(1024) normLongRows(NormArgs a) {
+  __shared__ float lds[16];
+  const uint32_t row = blockIdx.x;
+  const uint32_t steps = (a.cols + 1024 * 8 - 1) / (1024 * 8);
+  float q = 0.f;
+  for (uint32_t s = 0; s < steps; s++) {
+    const uint32_t c[1] = {(s * 1024 + threadIdx.x) * 8};
+    float f[1][8];
+    sumInputs<T, 1, 8>(a, row, c, f);
+#pragma unroll
+    for (int j = 0; j < 8; j++) q = __builtin_fmaf(f[0][j], f[0][j], q);
+  }
+  q = blockSum(q, lds, 16);
+  const float r = 1.f / sqrtf(q / (float)a.cols + a.eps);
+  for (uint32_t s = 0; s < steps; s++) {
+    const uint32_t c[1] = {(s * 1024 + threadIdx.x) * 8};
+    float f[1][8];
+    sumInputs<T, 1, 8>(a, row, c, f);
+    finishOctet<T, QUANT>(a, row, c[0], f[0], r);
+  }
+}
+
+// ------------------------------------------------------------------ gradients
+
+struct NormGradArgs {
+  const void *dy, *x, *dtotal, *weight;
+  void *dx;
+  float *partial;                             // [gridDim.x * rows at a time][cols] sums of dweight, or NULL
+  float *rms;                                 // long rows: 1 / rms per row for the column kernel
+  size_t ldDy, ldX, ldDtotal, ldDx;
+  uint32_t rows, cols;
+  float eps;
+  uint32_t weightF32;
+};
+
+template <class T>
+__device__ __forceinline__ void gradWeights(const NormGradArgs &a, uint32_t c, float (&w)[8]) {
+  NormArgs n;
+  n.weight = a.weight;
+  n.weightF32 = a.weightF32;
+  n.cols = a.cols;
+  weights<T>(n, c, w);
+}
+
+template <class T, int V>
+struct GradRow {
+  Octet<T> x[V], dy[V], dt[V];
+  __device__ __forceinline__ void load(const NormGradArgs &a, uint32_t row, const uint32_t (&c)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      x[i] = loadOctet((const T *)a.x + (size_t)row * a.ldX, c[i], a.cols);
+      dy[i] = loadOctet((const T *)a.dy + (size_t)row * a.ldDy, c[i], a.cols);
+    }
+    if (a.dtotal && a.dx)
+#pragma unroll
+      for (int i = 0; i < V; i++) dt[i] = loadOctet((const T *)a.dtotal + (size_t)row * a.ldDtotal, c[i], a.cols);
+  }
+};
+
+// A workgroup walks rows blockIdx.x, blockIdx.x + gridDim.x, ... (per TPR threads),
+// keeps its columns' share of dweight in registers and stores it once at the end.
+template <class T, int TPR, int V>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) normGradRows(NormGradArgs a) {
+  constexpr uint32_t kPer = TPR < 256 ? 256 / TPR : 1;
+  __shared__ float lds[2][16];
+  const uint32_t lane = threadIdx.x % TPR, slot = blockIdx.x * kPer + threadIdx.x / TPR;
+  uint32_t c[V];
+  float w[V][8], dw[V][8];
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    c[i] = (i * TPR + lane) * 8;
+    gradWeights<T>(a, c[i], w[i]);
+#pragma unroll
+    for (int j = 0; j < 8; j++) dw[i][j] = 0.f;
+  }
+  const float invC = 1.f / (float)a.cols;
+  for (uint32_t row = slot; row < a.rows; row += gridDim.x * kPer) {
+    GradRow<T, V> g;
+    g.load(a, row, c);
+    float q = 0.f, m = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; i++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float x = g.x[i].get(j);
+        q = __builtin_fmaf(x, x, q);
+        m = __builtin_fmaf(g.dy[i].get(j) * w[i][j], x, m);
+      }
+    q = waveSum(q);
+    m = waveSum(m);
+    if constexpr (TPR > 64) {
+      __syncthreads();                        // the row before has been read by everybody
+      if ((threadIdx.x & 63) == 0) {
+        lds[0][threadIdx.x >> 6] = q;
+        lds[1][threadIdx.x >> 6] = m;
+      }
+      __syncthreads();
+      q = m = 0.f;
+#pragma unroll
+      for (int s = 0; s < TPR / 64; s++) {
+        q += lds[0][s];
+        m += lds[1][s];
+      }
+    }
+    const float r = 1.f / sqrtf(q * invC + a.eps);
+    const float h = m * invC * r * r;         // mean(g xh) / rms: dx = r (g - x h)
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      float d[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float x = g.x[i].get(j), dy = g.dy[i].get(j);
+        dw[i][j] = __builtin_fmaf(dy, x * r, dw[i][j]);
+        d[j] = r * __builtin_fmaf(-x, h, dy * w[i][j]);
+        if (a.dtotal) d[j] += g.dt[i].get(j);
+      }
+      if (a.dx) storeOctet((T *)a.dx + (size_t)row * a.ldDx, c[i], a.cols, d);
+    }
+  }
+  if (a.partial)
+#pragma unroll
+    for (int i = 0; i < V; i++) storeOctet(a.partial + (size_t)slot * a.cols, c[i], a.cols, dw[i]);
+}
+
+template <class T>
+__global__ void __launch_bounds__(1024) normGradLongRows(NormGradArgs a) {
+  __shared__ float lds[16];
+  const uint32_t row = blockIdx.x;
+  const uint32_t steps = (a.cols + 1024 * 8 - 1) / (1024 * 8);
+  float q = 0.f, m = 0.f;
+  for (uint32_t s = 0; s < steps; s++) {
+    const uint32_t c[1] = {(s * 1024 + threadIdx.x) * 8};
+    GradRow<T, 1> g;
+    g.load(a, row, c);
+    float w[8];
+    gradWeights<T>(a, c[0], w);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float x = g.x[0].get(j);
+      q = __builtin_fmaf(x, x, q);
+      m = __builtin_fmaf(g.dy[0].get(j) * w[j], x, m);
+    }
+  }
+  q = blockSum(q, lds, 16);
+  m = blockSum(m, lds, 16);
+  const float invC = 1.f / (float)a.cols;
+  const float r = 1.f / sqrtf(q * invC + a.eps);
+  const float h = m * invC * r * r;
+  if (a.rms && threadIdx.x == 0) a.rms[row] = r;
+  if (!a.dx) return;
+  for (uint32_t s = 0; s < steps; s++) {
+    const uint32_t c[1] = {(s * 1024 + threadIdx.x) * 8};
+    GradRow<T, 1> g;
+    g.load(a, row, c);
+    float w[8], d[8];
+    gradWeights<T>(a, c[0], w);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      d[j] = r * __builtin_fmaf(-g.x[0].get(j), h, g.dy[0].get(j) * w[j]);
+      if (a.dtotal) d[j] += g.dt[0].get(j);
+    }
+    storeOctet((T *)a.dx + (size_t)row * a.ldDx, c[0], a.cols, d);
+  }
+}
+
+// Must run before dx is written when dx equals dy: it reads dy again.  Workgroup
+// (x, y): 2048 columns, every gridDim.y-th row from row y.
+template <class T>
+__global__ void __launch_bounds__(256) normGradLongColumns(NormGradArgs a) {
+  const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * 8;
+  float dw[8] = {};
+  for (uint32_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const Octet<T> x = loadOctet((const T *)a.x + (size_t)row * a.ldX, c, a.cols);
+    const Octet<T> dy = loadOctet((const T *)a.dy + (size_t)row * a.ldDy, c, a.cols);
+    const float r = a.rms[row];
+#pragma unroll
+    for (int j = 0; j < 8; j++) dw[j] = __builtin_fmaf(dy.get(j), x.get(j) * r, dw[j]);
+  }
+  storeOctet(a.partial + (size_t)blockIdx.y * a.cols, c, a.cols, dw);
+}
+
+// dweight = sum of `n` rows of partial sums, in a fixed order: 16 groups of rows
+// per 64 columns, joined through LDS.
+template <class W>
+__global__ void __launch_bounds__(256) normGradJoin(const float *partial, uint32_t n, uint32_t cols, W *dweight) {
+  __shared__ float lds[16][64];
+  const uint32_t part = threadIdx.x >> 4, c = blockIdx.x * 64 + (threadIdx.x & 15) * 4;
+  float s[4] = {};
+  for (uint32_t r = part; r < n; r += 16) {
+    const float *p = partial + (size_t)r * cols;
+    if (c + 4 <= cols) {
+      typedef float f32x4_anywhere __attribute__((ext_vector_type(4), aligned(4)));
+      const f32x4_anywhere v = *reinterpret_cast<const f32x4_anywhere *>(p + c);
+#pragma unroll
+      for (int j = 0; j < 4; j++) s[j] += v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (c + j < cols) s[j] += p[c + j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) lds[part][(threadIdx.x & 15) * 4 + j] = s[j];
+  __syncthreads();
+  if (threadIdx.x < 64 && blockIdx.x * 64 + threadIdx.x < cols) {
+    float t = 0.f;
+#pragma unroll
+    for (int p = 0; p < 16; p++) t += lds[p][threadIdx.x];
+    dweight[blockIdx.x * 64 + threadIdx.x] = (W)t;
+  }
+}
+
+// ----------------------------------------------------------------- host side
+
+template <class... P, class... A>
+flagcxResult_t launchShape(void (*kernel)(P...), dim3 grid, uint32_t block, hipStream_t s, const A &...args) {
+  std::tuple<P...> vals{static_cast<P>(args)...};
+  void *argv[sizeof...(P)];
+  argPointers(vals, argv, std::index_sequence_for<P...>{});
+  return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, dim3(block), argv, 0, s) == hipSuccess
+             ? flagcxSuccess
+             : flagcxUnhandledDeviceError;
+}
+
+size_t elementSize(int dt) {
+  return dt == FX_E4M3 ? 1 : (dt == flagcxBfloat16 || dt == flagcxFloat16) ? 2 : dt == flagcxFloat32 ? 4 : 0;
+}
+bool known(int dt) { return (dt >= 0 && dt < flagcxNumTypes) || dt == FX_E4M3; }
+bool at(const void *p, size_t es) { return p && ((uintptr_t)p & (es - 1)) == 0; }
+
+// dtype / weight_dtype of both entry points
+flagcxResult_t screenTypes(int dtype, int weightDtype) {
+  if (!known(dtype) || !known(weightDtype)) return flagcxInvalidArgument;
+  if (dtype == FX_E4M3 || !elementSize(dtype)) return flagcxNotSupported;
+  if (weightDtype != dtype && weightDtype != flagcxFloat32) return flagcxNotSupported;
+  return flagcxSuccess;
+}
+
+constexpr size_t kMaxExtent = 0x7fffffff;
+
+template <class T, bool QUANT>
+flagcxResult_t launchNorm(const NormArgs &a, hipStream_t s) {
+  const uint32_t octets = (a.cols + 7) / 8;
+  auto go = [&](auto kernel, uint32_t tpr) {
+    const uint32_t per = tpr < 256 ? 256 / tpr : 1;
+    return launchShape(kernel, dim3((a.rows + per - 1) / per), tpr < 256 ? 256 : tpr, s, a);
+  };
+  if (a.cols > kHeld) return launchShape(normLongRows<T, QUANT>, dim3(a.rows), 1024, s, a);
+  if (octets <= 64) return go(normRows<T, 64, 1, QUANT>, 64);
+  if (octets <= 128) return go(normRows<T, 64, 2, QUANT>, 64);
+  if (octets <= 256) return go(normRows<T, 256, 1, QUANT>, 256);
+  if (octets <= 512) return go(normRows<T, 256, 2, QUANT>, 256);
+  if (octets <= 1024) return go(normRows<T, 256, 4, QUANT>, 256);
+  if (octets <= 2048) return go(normRows<T, 512, 4, QUANT>, 512);
+  return go(normRows<T, 1024, 4, QUANT>, 1024);
+}
+
+template <class T>
+flagcxResult_t launchNormOut(const NormArgs &a, bool quant, hipStream_t s) {
+  return quant ? launchNorm<T, true>(a, s) : launchNorm<T, false>(a, s);
+}
+
+// Rows of partial sums of dweight.  Two workgroups per CU keep the loads busy;
+// fewer when there are fewer rows.
+constexpr uint32_t kGradWgs = 512;
+constexpr uint32_t kLongParts = 64;
+
+struct GradShape {
+  uint32_t tpr, v, wgs, parts;
+};
+GradShape gradShape(size_t rows, size_t cols) {
+  const size_t octets = (cols + 7) / 8;
+  GradShape g;
+  if (octets <= 64) g = {64, 1, 0, 0};
+  else if (octets <= 128) g = {64, 2, 0, 0};
+  else if (octets <= 256) g = {256, 1, 0, 0};
+  else if (octets <= 512) g = {256, 2, 0, 0};
+  else if (octets <= 1024) g = {256, 4, 0, 0};
+  else if (octets <= 2048) g = {512, 4, 0, 0};
+  else g = {1024, 4, 0, 0};
+  const size_t per = g.tpr < 256 ? 256 / g.tpr : 1;
+  const size_t want = (rows + per - 1) / per;
+  g.wgs = (uint32_t)(want < kGradWgs ? want : kGradWgs);
+  g.parts = g.wgs * (uint32_t)per;
+  return g;
+}
+
+template <class T>
+flagcxResult_t launchGradRows(const NormGradArgs &a, const GradShape &g, hipStream_t s) {
+  auto go = [&](auto kernel) { return launchShape(kernel, dim3(g.wgs), g.tpr < 256 ? 256 : g.tpr, s, a); };
+  switch (g.tpr * 8 + g.v) {
+    case 64 * 8 + 1: return go(normGradRows<T, 64, 1>);
+    case 64 * 8 + 2: return go(normGradRows<T, 64, 2>);
+    case 256 * 8 + 1: return go(normGradRows<T, 256, 1>);
+    case 256 * 8 + 2: return go(normGradRows<T, 256, 2>);
+    case 256 * 8 + 4: return go(normGradRows<T, 256, 4>);
+    case 512 * 8 + 4: return go(normGradRows<T, 512, 4>);
+    default: return go(normGradRows<T, 1024, 4>);
+  }
+}
+
+template <class T>
+flagcxResult_t launchGrad(NormGradArgs a, void *dweight, bool weightF32, void *workspace, hipStream_t s) {
+  uint32_t parts = 0;
+  flagcxResult_t rc = flagcxSuccess;
+  a.partial = dweight ? (float *)workspace : nullptr;
+  a.rms = nullptr;
+  if (a.rows && a.cols > kHeld) {
+    // The column kernel reads dy and x again, so it goes before the pass that writes dx (which may equal dy):
+    // rms first, without dx; then the columns; then dx.
+    if (dweight) {
+      parts = a.rows < kLongParts ? a.rows : kLongParts;
+      a.rms = (float *)workspace + (size_t)kLongParts * a.cols;
+      NormGradArgs b = a;
+      b.dx = nullptr;
+      rc = launchShape(normGradLongRows<T>, dim3(a.rows), 1024, s, b);
+      if (rc != flagcxSuccess) return rc;
+      rc = launchShape(normGradLongColumns<T>, dim3((a.cols + 2047) / 2048, parts), 256, s, b);
+      if (rc != flagcxSuccess) return rc;
+    }
+    if (a.dx) rc = launchShape(normGradLongRows<T>, dim3(a.rows), 1024, s, a);
+  } else if (a.rows) {
+    const GradShape g = gradShape(a.rows, a.cols);
+    parts = g.parts;
+    rc = launchGradRows<T>(a, g, s);
+  }
+  if (rc != flagcxSuccess || !dweight) return rc;
+  const dim3 grid((a.cols + 63) / 64);
+  if (weightF32) return launchShape(normGradJoin<float>, grid, 256, s, (const float *)workspace, parts, a.cols, (float *)dweight);
+  return launchShape(normGradJoin<T>, grid, 256, s, (const float *)workspace, parts, a.cols, (T *)dweight);
+}
+
+}  // namespace
+
+extern "C" {
+#pragma GCC visibility push(default)
+
+int fx_reduce_norm(void *out, float *scale, void *total, const void *const *in, int k, const void *residual,
+                   const void *weight, size_t rows, size_t cols, const fxNormStrides *strides, int dtype,
+                   int weight_dtype, int out_dtype, float eps, void *stream) {
+  const flagcxResult_t rc = screenTypes(dtype, weight_dtype);
+  if (rc != flagcxSuccess) return rc;
+  if (!known(out_dtype)) return flagcxInvalidArgument;
+  if (out_dtype != dtype && out_dtype != FX_E4M3) return flagcxNotSupported;
+  if (!in || k < 1 || k > FX_MAX_INPUTS || rows > kMaxExtent || cols > kMaxExtent || !(eps >= 0.f)) return flagcxInvalidArgument;
+  const bool quant = out_dtype == FX_E4M3;
+  if (quant != (scale != nullptr)) return flagcxInvalidArgument;
+  if (rows == 0 || cols == 0) return flagcxSuccess;
+  const size_t es = elementSize(dtype), groups = (cols + FX_SCALE_GROUP - 1) / FX_SCALE_GROUP;
+  const fxNormStrides st = strides ? *strides : fxNormStrides{cols, cols, cols, cols, groups};
+  if (st.in < cols || st.out < cols || (residual && st.residual < cols) || (total && st.total < cols) || (quant && st.scale < groups))
+    return flagcxInvalidArgument;
+  if (!at(out, quant ? 1 : es) || (total && !at(total, es)) || (residual && !at(residual, es)) ||
+      (weight && !at(weight, elementSize(weight_dtype))) || (quant && !at(scale, 4)))
+    return flagcxInvalidArgument;
+  NormArgs a;
+  for (int p = 0; p < k; p++) {
+    if (!at(in[p], es)) return flagcxInvalidArgument;
+    a.in[p] = in[p];
+  }
+  for (int p = k; p <= FX_MAX_INPUTS; p++) a.in[p] = residual;
+  a.total = total;
+  a.out = out;
+  a.scale = scale;
+  a.weight = weight;
+  a.ldIn = st.in;
+  a.ldRes = st.residual;
+  a.ldTotal = st.total;
+  a.ldOut = st.out;
+  a.ldScale = st.scale;
+  a.rows = (uint32_t)rows;
+  a.cols = (uint32_t)cols;
+  a.k = (uint32_t)k;
+  a.n = (uint32_t)k + (residual ? 1 : 0);
+  a.eps = eps;
+  a.weightF32 = weight_dtype == flagcxFloat32;
+  hipStream_t s = (hipStream_t)stream;
+  switch (dtype) {
+    case flagcxBfloat16: return launchNormOut<__bf16>(a, quant, s);
+    case flagcxFloat16: return launchNormOut<_Float16>(a, quant, s);
+    default: return launchNormOut<float>(a, quant, s);
+  }
+}
+
+size_t fx_reduce_norm_grad_workspace(size_t rows, size_t cols) {
+  if (rows == 0 || cols == 0) return 0;
+  if (cols > kHeld) return ((size_t)kLongParts * cols + rows) * sizeof(float);
+  return (size_t)gradShape(rows, cols).parts * cols * sizeof(float);
+}
+
+int fx_reduce_norm_grad(void *dx, void *dweight, const void *dy, const void *x, const void *dtotal, const void *weight,
+                        size_t rows, size_t cols, const fxNormGradStrides *strides, int dtype, int weight_dtype, float eps,
+                        void *workspace, size_t workspace_bytes, void *stream) {
+  const flagcxResult_t rc = screenTypes(dtype, weight_dtype);
+  if (rc != flagcxSuccess) return rc;
+  if (rows > kMaxExtent || cols > kMaxExtent || !(eps >= 0.f)) return flagcxInvalidArgument;
+  if (cols == 0 || (!dx && !dweight)) return flagcxSuccess;
+  const size_t es = elementSize(dtype);
+  if (dweight && !at(dweight, elementSize(weight_dtype))) return flagcxInvalidArgument;
+  const fxNormGradStrides st = strides ? *strides : fxNormGradStrides{cols, cols, cols, cols};
+  if (rows) {
+    if (!at(dy, es) || !at(x, es) || (dx && !at(dx, es)) || (dtotal && !at(dtotal, es)) ||
+        (weight && !at(weight, elementSize(weight_dtype))))
+      return flagcxInvalidArgument;
+    if (st.dy < cols || st.x < cols || (dtotal && st.dtotal < cols) || (dx && st.dx < cols)) return flagcxInvalidArgument;
+    if (dweight && (!at(workspace, 16) || workspace_bytes < fx_reduce_norm_grad_workspace(rows, cols)))
+      return flagcxInvalidArgument;
+  }
+  NormGradArgs a;
+  a.dy = dy;
+  a.x = x;
+  a.dtotal = dtotal;
+  a.weight = weight;
+  a.dx = dx;
+  a.ldDy = st.dy;
+  a.ldX = st.x;
+  a.ldDtotal = st.dtotal;
+  a.ldDx = st.dx;
+  a.rows = (uint32_t)rows;
+  a.cols = (uint32_t)cols;
+  a.eps = eps;
+  a.weightF32 = weight_dtype == flagcxFloat32;
+  hipStream_t s = (hipStream_t)stream;
+  if (rows == 0 && !dweight) return flagcxSuccess;
+  switch (dtype) {
+    case flagcxBfloat16: return launchGrad<__bf16>(a, dweight, a.weightF32, workspace, s);
+    case flagcxFloat16: return launchGrad<_Float16>(a, dweight, a.weightF32, workspace, s);
+    default: return launchGrad<float>(a, dweight, a.weightF32, workspace, s);
+  }
+}
+
+#pragma GCC visibility pop
+}

@@ -1,0 +1,483 @@
+// Matrix products grouped by expert on the matrix cores: the tiled kernel.
+//
+// A workgroup computes a BN x BM tile of the output (n = contiguous columns of
+// the output, m = its rows) and walks the reduction in slabs of 128 bytes per row
+// (64 elements of 16 bits, 128 of 8).  The matrix instruction takes the n side as
+// its first operand, so that a lane's accumulators are consecutive columns of one
+// output row: stores are vectors and a row's scale is one value per lane.
+//
+// Each operand is either held with the reduction contiguous ("along") or with its
+// own index contiguous ("across"):
+//                      n side            m side
+//   y  = x W^T  (NK)   w, along          x, along
+//   y  = x W    (KN)   w, across         x, along
+//   dw = dy^T x        x, across         dy, across
+// An "along" tile lies in LDS as rows of 128 bytes whose eight 16-byte chunks are
+// exchanged by a function of the row, so that the eight lanes that a 128-bit read
+// serves at a time meet eight different chunks.  An "across" tile keeps its rows
+// of the reduction and is read with the transposing LDS loads, four rows by 32
+// bytes at a time; its 32-byte units are exchanged by the row's two low bits.
+#pragma once
+#include "flagcx_amd/fx_model.h"
+#include "fx_vec.hpp"
+
+namespace fx {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+struct E4m3 {};        // 8-bit matrix instructions (their sums over 128 carry about 16 bits)
+struct E4m3Exact {};   // widened to bf16 first: sums as in fp32, half the rate
+
+template <class T>
+constexpr int kBytes = 2;
+template <>
+inline constexpr int kBytes<E4m3> = 1;
+template <>
+inline constexpr int kBytes<E4m3Exact> = 1;
+
+struct ProductArgs {
+  const void *pn, *pm;             // operands of the n side and the m side
+  void *y;
+  const float *sn, *sm;            // e4m3: scales of the n side (blocks) and of the m side (rows)
+  const int32_t *offsets;
+  size_t ldn, ldm, ldy;            // elements
+  size_t expertN, expertY;         // products: weights' stride; dw: output's stride
+  size_t ldsn, ldsm, expertSn;
+  uint32_t experts, rows;
+  uint32_t n, m, k;                // output columns; dw: output rows; products: length of the reduction
+  uint32_t mTiles, nTiles;         // products: upper bound of row tiles over all experts; dw: per expert
+};
+
+// What one workgroup computes.
+struct Tile {
+  uint32_t expert, m0, mEnd, n0, k0, kLen;   // rows [m0, mEnd) of the m side; reduction [k0, k0 + kLen)
+};
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+// Expert boundaries as the kernels use them: never outside [0, rows].
+__device__ __forceinline__ uint32_t bound(const ProductArgs &a, uint32_t e) {
+  const int32_t o = a.offsets[e];
+  return o < 0 ? 0u : ((uint32_t)o > a.rows ? a.rows : (uint32_t)o);
+}
+
+__device__ __forceinline__ uint32_t waveScan(uint32_t v) {   // inclusive prefix sum over the wavefront
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_up((int)v, d);
+    if ((int)(threadIdx.x & 63) >= d) v += o;
+  }
+  return v;
+}
+
+// Tiles of BM rows that expert e's rows make.
+template <int BM>
+__device__ __forceinline__ uint32_t tilesOf(const ProductArgs &a, uint32_t e, uint32_t *first, uint32_t *last) {
+  *first = *last = 0;
+  if (e >= a.experts) return 0;
+  *first = bound(a, e);
+  *last = bound(a, e + 1);
+  return *last > *first ? (*last - *first + BM - 1) / BM : 0;
+}
+
+// Consecutive tiles of one die (workgroups go to the eight dies in turn) are made
+// neighbours: a die's L2 then holds the operands of a block of kPanel row tiles by
+// a few column tiles.
+constexpr uint32_t kDies = 8, kPanel = 8;
+__device__ __forceinline__ uint32_t dieOrder(uint32_t id, uint32_t total) {
+  const uint32_t die = id % kDies, at = id / kDies, q = total / kDies, r = total % kDies;
+  return die * q + (die < r ? die : r) + at;
+}
+__device__ __forceinline__ void panelOrder(uint32_t id, uint32_t mTiles, uint32_t nTiles, uint32_t *mt, uint32_t *nt) {
+  const uint32_t panel = id / (kPanel * nTiles), rem = id - panel * kPanel * nTiles;
+  const uint32_t left = mTiles - panel * kPanel, h = left < kPanel ? left : kPanel;
+  *mt = panel * kPanel + rem % h;
+  *nt = rem / h;
+}
+
+// The row tiles of all experts are counted on the device (the host knows only an
+// upper bound, the grid): every wavefront scans the boundaries, 64 experts at a time.
+template <int BN, int BM>
+__device__ __forceinline__ bool findTile(const ProductArgs &a, Tile *t) {
+  uint32_t mTiles, mt, nt;
+  if (!a.offsets) {
+    mTiles = (a.rows + BM - 1) / BM;
+    if (blockIdx.x >= mTiles * a.nTiles) return false;
+    panelOrder(dieOrder(blockIdx.x, mTiles * a.nTiles), mTiles, a.nTiles, &mt, &nt);
+    *t = Tile{0, mt * BM, a.rows, nt * BN, 0, a.k};
+    return true;
+  }
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t first, last, scan = 0;
+  mTiles = 0;
+  for (uint32_t e = 0; e < a.experts; e += 64) {
+    scan = waveScan(tilesOf<BM>(a, e + lane, &first, &last));
+    mTiles += uniform((uint32_t)__shfl((int)scan, 63));
+  }
+  if (mTiles > a.mTiles) mTiles = a.mTiles;          // boundaries that are not ascending: the grid ends here
+  if (blockIdx.x >= mTiles * a.nTiles) return false;
+  panelOrder(dieOrder(blockIdx.x, mTiles * a.nTiles), mTiles, a.nTiles, &mt, &nt);
+  uint32_t before = 0;
+  for (uint32_t e = 0; e < a.experts; e += 64) {
+    if (a.experts > 64) scan = waveScan(tilesOf<BM>(a, e + lane, &first, &last));
+    const uint32_t all = uniform((uint32_t)__shfl((int)scan, 63));
+    if (mt < before + all) {
+      const uint64_t over = __ballot(before + scan > mt);
+      const uint32_t l = (uint32_t)__builtin_ctzll(over);
+      const uint32_t prev = l ? uniform((uint32_t)__shfl((int)scan, (int)(l - 1))) : 0;
+      const uint32_t f = uniform((uint32_t)__shfl((int)first, (int)l));
+      *t = Tile{e + l, f + (mt - before - prev) * BM, uniform((uint32_t)__shfl((int)last, (int)l)), nt * BN, 0, a.k};
+      return true;
+    }
+    before += all;
+  }
+  return false;
+}
+
+template <int BN, int BM>
+__device__ __forceinline__ bool findTileDw(const ProductArgs &a, Tile *t) {
+  const uint32_t per = a.mTiles * a.nTiles;
+  const uint32_t id = dieOrder(blockIdx.x, per * a.experts), e = id / per;
+  uint32_t mt, nt, first = 0, last = a.rows;
+  panelOrder(id - e * per, a.mTiles, a.nTiles, &mt, &nt);
+  if (a.offsets) {
+    first = uniform(bound(a, e));
+    last = uniform(bound(a, e + 1));
+  }
+  *t = Tile{e, mt * BM, a.m, nt * BN, first, last > first ? last - first : 0};
+  return true;
+}
+
+// ------------------------------------------------------- one operand's tile
+
+// Chunk exchange of an "along" tile.  On the m side the sixteen lanes of a
+// fragment are rows 16 f + i; on the n side rows 16 (i / 4) + 4 f + i % 4 of a
+// block of 64, which gives a lane sixteen consecutive columns over its four
+// fragments.
+template <bool NSIDE>
+__device__ __forceinline__ uint32_t exchange(uint32_t r) {
+  return NSIDE ? ((r & 3) | ((r >> 2) & 4)) : (r & 7);
+}
+
+// R = extent of the tile in its own index, NT = threads, ES = bytes per element.
+template <int R, int NT, int ES, bool ACROSS, bool NSIDE>
+struct Side {
+  static constexpr int kLoads = R * 8 / NT;              // 16-byte chunks per thread and slab
+  static constexpr int kPerRow = ACROSS ? R / 8 : 8;     // chunks per LDS row
+  static constexpr int kStep = NT / kPerRow;             // rows between a thread's chunks
+  static constexpr int kElems = 16 / ES;
+  static constexpr uint32_t kSlab = 128 / ES;            // reduction elements per slab
+
+  // position of this thread's first chunk
+  uint32_t row, chunk;
+  __device__ __forceinline__ void init() {
+    row = threadIdx.x / kPerRow;
+    const uint32_t p = threadIdx.x % kPerRow;
+    chunk = ACROSS ? ((((p >> 1) ^ (row & 3)) << 1) | (p & 1)) : (p ^ exchange<NSIDE>(row));
+  }
+
+  // One chunk, element by element where it is not whole; `base` = the tile's own
+  // index 0 at reduction 0.  own / red: how much of the tile's own index and of the
+  // slab's reduction exists.
+  __device__ __forceinline__ u32x4 guarded(const char *base, size_t ld, int i, uint32_t own, uint32_t red) const {
+    const uint32_t r = row + i * kStep, c = chunk * kElems;
+    u32x4 v = {};
+    const uint32_t rows = ACROSS ? red : own, cols = ACROSS ? own : red;
+    if (r >= rows || c >= cols) return v;
+    const char *p = base + ((size_t)r * ld + c) * ES;
+    if (c + kElems <= cols) return *reinterpret_cast<const u32x4_anywhere *>(p);
+    if constexpr (ES == 2) {
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (c + j < cols) v[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[j] << (16 * (j & 1));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (c + j < cols) v[j >> 2] |= (uint32_t) reinterpret_cast<const uint8_t *>(p)[j] << (8 * (j & 3));
+    }
+    return v;
+  }
+};
+
+// Fragment reads.  lane l: index i = l % 16 of the fragment, reduction group g = l / 16.
+template <bool NSIDE>
+__device__ __forceinline__ u32x4 readAlong(const char *lds, uint32_t wave0, int f, int half, uint32_t i, uint32_t g) {
+  const uint32_t r = NSIDE ? wave0 + (f >> 2) * 64 + 16 * (i >> 2) + 4 * (f & 3) + (i & 3) : wave0 + 16 * f + i;
+  return *reinterpret_cast<const u32x4 *>(lds + r * 128 + (((uint32_t)(half * 4) + g) ^ exchange<NSIDE>(r)) * 16);
+}
+template <int R>
+__device__ __forceinline__ u32x4 readAcross(const char *lds, uint32_t wave0, int f, int half, uint32_t i, uint32_t g) {
+  typedef __attribute__((address_space(3))) s16x4 *lds64;
+  const uint32_t unit = (wave0 + 16 * f) / 16;
+  const uint32_t k = 32 * half + 8 * g + (i >> 2);
+  const uint32_t at = k * (R * 2) + ((unit ^ (i >> 2)) * 32) + (i & 3) * 8;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds64)(lds + at));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds64)(lds + at + 4 * R * 2));
+  const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
+  return u32x4{x[0], x[1], y[0], y[1]};
+}
+
+// eight e4m3 codes (two words) as bf16: exact
+__device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+template <class T>
+__device__ __forceinline__ f32x4 mma(u32x4 n, u32x4 m, f32x4 c) {
+  if constexpr (__is_same(T, __bf16))
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, n), __builtin_bit_cast(bf16x8, m), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, n), __builtin_bit_cast(f16x8, m), c, 0, 0, 0);
+}
+
+// 128 products of e4m3 values: two chunks per side
+template <class T>
+__device__ __forceinline__ f32x4 mma8(const u32x4 (&n)[2], const u32x4 (&m)[2]) {
+  f32x4 c = {};
+  if constexpr (__is_same(T, E4m3)) {
+    const i32x8 a = {(int)n[0][0], (int)n[0][1], (int)n[0][2], (int)n[0][3], (int)n[1][0], (int)n[1][1], (int)n[1][2], (int)n[1][3]};
+    const i32x8 b = {(int)m[0][0], (int)m[0][1], (int)m[0][2], (int)m[0][3], (int)m[1][0], (int)m[1][1], (int)m[1][2], (int)m[1][3]};
+    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(n[h][0], n[h][1]), widen(m[h][0], m[h][1]), c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(n[h][2], n[h][3]), widen(m[h][2], m[h][3]), c, 0, 0, 0);
+    }
+  }
+  return c;
+}
+
+// N consecutive columns of one output row
+template <class Out, int N>
+__device__ __forceinline__ void storeRun(Out *p, uint32_t c, uint32_t cols, const float (&f)[N]) {
+  if (c + N <= cols) {
+    if constexpr (sizeof(Out) == 4) {
+#pragma unroll
+      for (int q = 0; q < N / 4; q++) {
+        u32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = __builtin_bit_cast(uint32_t, f[4 * q + j]);
+        *reinterpret_cast<u32x4_anywhere *>(p + c + 4 * q) = v;
+      }
+    } else {
+      typedef uint32_t words __attribute__((ext_vector_type(N / 2 < 4 ? N / 2 : 4), aligned(1)));
+      constexpr int W = N / 2 < 4 ? N / 2 : 4;
+#pragma unroll
+      for (int q = 0; q < N / (2 * W); q++) {
+        words v;
+#pragma unroll
+        for (int j = 0; j < W; j++)
+          v[j] = (uint32_t)__builtin_bit_cast(uint16_t, (Out)f[2 * W * q + 2 * j]) |
+                 ((uint32_t)__builtin_bit_cast(uint16_t, (Out)f[2 * W * q + 2 * j + 1]) << 16);
+        *reinterpret_cast<words *>(p + c + 2 * W * q) = v;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j++)
+      if (c + j < cols) p[c + j] = (Out)f[j];
+  }
+}
+
+// ---------------------------------------------------------------- the kernel
+
+// WN x WM wavefronts, each with a (BN / WN) x (BM / WM) part of the tile.
+template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW>
+struct Product {
+  static constexpr int kThreads = WN * WM * 64, ES = kBytes<T>;
+  static constexpr int TN = BN / WN, TM = BM / WM, FN = TN / 16, FM = TM / 16;
+  static constexpr bool kScaled = ES == 1;
+  static_assert(TN % 64 == 0 && TM % 16 == 0, "whole fragments");
+  using N = Side<BN, kThreads, ES, NACROSS, true>;
+  using M = Side<BM, kThreads, ES, MACROSS, false>;
+  static constexpr uint32_t kSlab = N::kSlab;
+  static constexpr int kLdsN = BN * 128, kLdsM = BM * 128;
+
+  f32x4 acc[FN][FM];
+  uint32_t i, g, wn, wm;
+
+  __device__ __forceinline__ void init() {
+    const uint32_t wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    i = lane & 15;
+    g = lane >> 4;
+    wn = (wave % WN) * TN;
+    wm = (wave / WN) * TM;
+#pragma unroll
+    for (int f = 0; f < FN; f++)
+#pragma unroll
+      for (int h = 0; h < FM; h++) acc[f][h] = f32x4{};
+  }
+
+  __device__ __forceinline__ u32x4 readN(const char *lds, int f, int half) const {
+    if constexpr (NACROSS) return readAcross<BN>(lds, wn, f, half, i, g);
+    else return readAlong<true>(lds, wn, f, half, i, g);
+  }
+  __device__ __forceinline__ u32x4 readM(const char *lds, int f, int half) const {
+    if constexpr (MACROSS) return readAcross<BM>(lds, wm, f, half, i, g);
+    else return readAlong<false>(lds, wm, f, half, i, g);
+  }
+
+  // One slab from LDS.  scale: this slab's m-side scale per fragment, times the n side's
+  __device__ __forceinline__ void slab(const char *ln, const char *lm, const float (&scale)[FM]) {
+    if constexpr (kScaled) {
+      u32x4 n[FN][2];
+#pragma unroll
+      for (int f = 0; f < FN; f++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) n[f][h] = readN(ln, f, h);
+#pragma unroll
+      for (int q = 0; q < FM; q++) {
+        const u32x4 m[2] = {readM(lm, q, 0), readM(lm, q, 1)};
+#pragma unroll
+        for (int f = 0; f < FN; f++) {
+          const f32x4 p = mma8<T>(n[f], m);
+#pragma unroll
+          for (int v = 0; v < 4; v++) acc[f][q][v] = __builtin_fmaf(p[v], scale[q], acc[f][q][v]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        u32x4 n[FN];
+#pragma unroll
+        for (int f = 0; f < FN; f++) n[f] = readN(ln, f, h);
+#pragma unroll
+        for (int q = 0; q < FM; q++) {
+          const u32x4 m = readM(lm, q, h);
+#pragma unroll
+          for (int f = 0; f < FN; f++) acc[f][q] = mma<T>(n[f], m, acc[f][q]);
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void store(const ProductArgs &a, const Tile &t) const {
+    Out *y = (Out *)a.y + (DW ? (size_t)t.expert * a.expertY : 0);
+#pragma unroll
+    for (int q = 0; q < FM; q++) {
+      const uint32_t m = t.m0 + wm + 16 * q + i;
+      if (m >= t.mEnd) continue;
+      Out *row = y + (size_t)m * a.ldy;
+      if constexpr (NACROSS) {
+#pragma unroll
+        for (int f = 0; f < FN; f++) {
+          const float v[4] = {acc[f][q][0], acc[f][q][1], acc[f][q][2], acc[f][q][3]};
+          storeRun(row, t.n0 + wn + 16 * f + 4 * g, a.n, v);
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < FN / 4; b++) {
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 16; j++) v[j] = acc[4 * b + (j >> 2)][q][j & 3];
+          storeRun(row, t.n0 + wn + 64 * b + 16 * g, a.n, v);
+        }
+      }
+    }
+  }
+
+  // m-side scales of slab s for this lane's rows, times the n side's block scale.
+  // A wavefront's 64 columns lie in one block of 128; columns and rows that do not
+  // exist take an existing scale (their products are not stored).
+  __device__ __forceinline__ void scales(const ProductArgs &a, const Tile &t, uint32_t s, float (&out)[FM]) const {
+    if constexpr (kScaled) {
+      static_assert(TN == 64, "one block scale per wavefront");
+      const uint32_t last = (a.n - 1) / FX_SCALE_GROUP, b = (t.n0 + wn) / FX_SCALE_GROUP;
+      const float sn = a.sn[(size_t)t.expert * a.expertSn + (size_t)(b < last ? b : last) * a.ldsn + s];
+#pragma unroll
+      for (int q = 0; q < FM; q++) {
+        const uint32_t m = t.m0 + wm + 16 * q + i;
+        out[q] = sn * a.sm[(size_t)(m < t.mEnd ? m : t.mEnd - 1) * a.ldsm + s];
+      }
+    }
+  }
+};
+
+// Any alignment and any sizes: chunks go through registers, and the next slab's
+// are on their way while this one is multiplied.
+template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW>
+__global__ void __launch_bounds__(WN *WM * 64) productGuarded(ProductArgs a) {
+  using P = Product<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>;
+  __shared__ __attribute__((aligned(1024))) char lds[P::kLdsN + P::kLdsM];
+  char *ln = lds, *lm = lds + P::kLdsN;
+  Tile t;
+  if (!(DW ? findTileDw<BN, BM>(a, &t) : findTile<BN, BM>(a, &t))) return;
+  P p;
+  p.init();
+  typename P::N sn;
+  typename P::M sm;
+  sn.init();
+  sm.init();
+  const size_t nAt = NACROSS ? (size_t)t.k0 * a.ldn + t.n0 : (size_t)t.n0 * a.ldn + t.k0;
+  const size_t mAt = MACROSS ? (size_t)t.k0 * a.ldm + t.m0 : (size_t)t.m0 * a.ldm + t.k0;
+  const char *bn = (const char *)a.pn + (nAt + (DW ? 0 : (size_t)t.expert * a.expertN)) * P::ES;
+  const char *bm = (const char *)a.pm + mAt * P::ES;
+  const uint32_t ownN = a.n - t.n0, ownM = t.mEnd - t.m0;
+  const uint32_t slabs = (t.kLen + P::kSlab - 1) / P::kSlab;
+  u32x4 vn[P::N::kLoads], vm[P::M::kLoads];
+  auto load = [&](uint32_t s) {
+    const uint32_t k = s * P::kSlab, red = t.kLen - k;
+    const char *pn = bn + (NACROSS ? (size_t)k * a.ldn : (size_t)k) * P::ES;
+    const char *pm = bm + (MACROSS ? (size_t)k * a.ldm : (size_t)k) * P::ES;
+#pragma unroll
+    for (int q = 0; q < P::N::kLoads; q++) vn[q] = sn.guarded(pn, a.ldn, q, ownN, red);
+#pragma unroll
+    for (int q = 0; q < P::M::kLoads; q++) vm[q] = sm.guarded(pm, a.ldm, q, ownM, red);
+  };
+  if (slabs) load(0);
+  for (uint32_t s = 0; s < slabs; s++) {
+    float scale[P::FM];
+    p.scales(a, t, s, scale);
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < P::N::kLoads; q++) *reinterpret_cast<u32x4 *>(ln + (q * P::kThreads + threadIdx.x) * 16) = vn[q];
+#pragma unroll
+    for (int q = 0; q < P::M::kLoads; q++) *reinterpret_cast<u32x4 *>(lm + (q * P::kThreads + threadIdx.x) * 16) = vm[q];
+    __syncthreads();
+    if (s + 1 < slabs) load(s + 1);
+    p.slab(ln, lm, scale);
+  }
+  p.store(a, t);
+}
+
+// ------------------------------------------------------------- launch tables
+
+enum ProductForm { kFormNK = 0, kFormKN = 1, kFormDw = 2 };
+
+// Implemented once per operand type (fx_product_*.hip).
+flagcxResult_t launchProductBf16(const ProductArgs &a, int form, bool outF32, hipStream_t s);
+flagcxResult_t launchProductF16(const ProductArgs &a, int form, bool outF32, hipStream_t s);
+flagcxResult_t launchProductE4m3(const ProductArgs &a, int outDtype, hipStream_t s);
+
+template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW>
+flagcxResult_t launchGuarded(ProductArgs a, hipStream_t s) {
+  a.nTiles = (a.n + BN - 1) / BN;
+  if (DW) a.mTiles = (a.m + BM - 1) / BM;
+  else if (!a.offsets) a.mTiles = (a.rows + BM - 1) / BM;
+  else a.mTiles = a.rows / BM + (a.experts < a.rows ? a.experts : a.rows);   // every expert's last tile may be partial
+  const uint64_t grid = (uint64_t)a.nTiles * a.mTiles * (DW ? a.experts : 1);
+  if (grid > 0x7fffffffu) return flagcxNotSupported;
+  void *argv[] = {&a};
+  const void *kernel = reinterpret_cast<const void *>(productGuarded<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
+  return hipLaunchKernel(kernel, dim3((uint32_t)grid), dim3(WN * WM * 64), argv, 0, s) == hipSuccess ? flagcxSuccess
+                                                                                                   : flagcxUnhandledDeviceError;
+}
+
+template <class T, class Out>
+flagcxResult_t launchForm(const ProductArgs &a, int form, hipStream_t s) {
+  switch (form) {
+    case kFormNK: return launchGuarded<T, Out, 128, 128, 2, 2, false, false, false>(a, s);
+    case kFormKN: return launchGuarded<T, Out, 128, 128, 2, 2, true, false, false>(a, s);
+    default: return launchGuarded<T, Out, 128, 128, 2, 2, true, true, true>(a, s);
+  }
+}
+
+}  // namespace fx

@@ -142,6 +142,49 @@ def unpack(recvbuff, packed, counts, displs, dtype, stream=None):
     return lib.fx_unpack(recvbuff, packed, _sz_array(counts), _sz_array(displs), len(counts), dtype, stream)
 
 
+# -- operators behind the collectives (include/flagcx_amd/fx_model.h); pointers are device addresses --
+
+W_NK, W_KN = 0, 1          # FX_WEIGHT_NK, FX_WEIGHT_KN
+
+
+def reduce_norm(out, ins, weight, rows, cols, dtype, *, eps, residual=None, total=None, scale=None, out_dtype=None,
+                weight_dtype=None, strides=None, stream=None):
+    """Sum of `ins`, residual addition and root-mean-square norm; out_dtype = N.DT_E4M3 also writes `scale`.
+    strides: dict of in_, residual, total, out, scale (elements from row to row), or None for dense rows."""
+    return lib.fx_reduce_norm(out, scale, total, _ptr_array(ins), len(ins), residual, weight, rows, cols, N.NormStrides.of(strides),
+                              dtype, dtype if weight_dtype is None else weight_dtype, dtype if out_dtype is None else out_dtype,
+                              eps, stream)
+
+
+def reduce_norm_grad_workspace(rows, cols):
+    return lib.fx_reduce_norm_grad_workspace(rows, cols)
+
+
+def reduce_norm_grad(dx, dweight, dy, x, weight, rows, cols, dtype, workspace, workspace_bytes, *, eps, dtotal=None,
+                     weight_dtype=None, strides=None, stream=None):
+    """Gradients of reduce_norm; x is what it stored as `total`.  dx or dweight may be None."""
+    return lib.fx_reduce_norm_grad(dx, dweight, dy, x, dtotal, weight, rows, cols, N.NormGradStrides.of(strides), dtype,
+                                   dtype if weight_dtype is None else weight_dtype, eps, workspace, workspace_bytes, stream)
+
+
+def expert_product(y, x, w, offsets, experts, rows, n, k, dtype, *, out_dtype=None, layout=W_NK, strides=None, stream=None):
+    """y = x W^T (W_NK) or x W (W_KN) with every expert's own weights; offsets: device int32[experts + 1] or None."""
+    return lib.fx_expert_product(y, x, w, offsets, experts, rows, n, k, layout, N.ProductStrides.of(strides), dtype,
+                                 dtype if out_dtype is None else out_dtype, stream)
+
+
+def expert_product_dw(dw, dy, x, offsets, experts, rows, n, k, dtype, *, out_dtype=None, strides=None, stream=None):
+    """dw[e] = dy_e^T x_e, [experts][n][k]."""
+    return lib.fx_expert_product_dw(dw, dy, x, offsets, experts, rows, n, k, N.ProductDwStrides.of(strides), dtype,
+                                    dtype if out_dtype is None else out_dtype, stream)
+
+
+def expert_product_e4m3(y, x, xscale, w, wscale, offsets, experts, rows, n, k, out_dtype, *, strides=None, stream=None):
+    """The product of e4m3 rows (a scale per 128 columns) and e4m3 weights (a scale per 128 x 128)."""
+    return lib.fx_expert_product_e4m3(y, x, xscale, w, wscale, offsets, experts, rows, n, k, N.ProductE4m3Strides.of(strides),
+                                      out_dtype, stream)
+
+
 def split(total, parts, idx):
     c, o = C.c_size_t(), C.c_size_t()
     lib.fx_split(total, parts, idx, C.byref(c), C.byref(o))

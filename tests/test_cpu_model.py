@@ -1,0 +1,184 @@
+"""The operators behind the collectives without a GPU: what they refuse, what they
+accept as nothing to do, and the gradients' formulas against differences."""
+import os
+import re
+import shutil
+import subprocess
+
+import numpy as np
+import pytest
+
+from flagcx_amd import _native as N
+from flagcx_amd import kernels as K
+from tests import model_ref as R
+
+P = 0x1000
+OK, BAD, NOT = N.SUCCESS, N.INVALID_ARGUMENT, N.NOT_SUPPORTED
+
+
+def norm(**kw):
+    a = dict(out=P, ins=[P, P], weight=P, rows=4, cols=256, dtype=N.DT_BF16, eps=1e-6, residual=P, total=P)
+    a.update(kw)
+    return K.reduce_norm(**a)
+
+
+def test_norm_refusals():
+    assert norm(dtype=N.DT_FP64) == NOT and norm(dtype=N.DT_INT32) == NOT and norm(dtype=N.DT_E4M3) == NOT
+    assert norm(dtype=10) == BAD and norm(dtype=-1) == BAD and norm(out_dtype=11) == BAD and norm(weight_dtype=77) == BAD
+    assert norm(out_dtype=N.DT_FP16) == NOT and norm(weight_dtype=N.DT_FP16) == NOT and norm(out_dtype=N.DT_FP32) == NOT
+    assert norm(ins=[]) == BAD and norm(ins=[P] * 65) == BAD and norm(ins=[P, None]) == BAD and norm(ins=[P + 1, P]) == BAD
+    assert norm(out=None) == BAD and norm(out=P + 1) == BAD and norm(total=P + 1) == BAD and norm(residual=P + 1) == BAD
+    assert norm(weight=P + 1) == BAD and norm(weight=P + 2, weight_dtype=N.DT_FP32) == BAD
+    assert norm(eps=-1.0) == BAD and norm(eps=float("nan")) == BAD
+    assert norm(out_dtype=N.DT_E4M3) == BAD                       # no scale
+    assert norm(scale=P) == BAD                                   # a scale nobody writes
+    assert norm(out_dtype=N.DT_E4M3, scale=P + 2) == BAD
+    wide = dict(in_=256, residual=256, total=256, out=256, scale=2)
+    for name in ("in_", "residual", "total", "out"):
+        assert norm(strides={**wide, name: 255}) == BAD
+    assert norm(out_dtype=N.DT_E4M3, scale=P, strides={**wide, "scale": 1}) == BAD
+    assert norm(rows=1 << 31) == BAD and norm(cols=1 << 31) == BAD
+    assert norm(rows=0, out=None, ins=[None]) == OK and norm(cols=0, out=None) == OK
+
+
+def grad(**kw):
+    a = dict(dx=P, dweight=P, dy=P, x=P, weight=P, rows=4, cols=256, dtype=N.DT_BF16, workspace=P, workspace_bytes=1 << 20,
+             eps=1e-6, dtotal=P)
+    a.update(kw)
+    return K.reduce_norm_grad(**a)
+
+
+def test_norm_gradient_refusals():
+    assert grad(dtype=N.DT_INT8) == NOT and grad(dtype=99) == BAD and grad(weight_dtype=N.DT_FP16) == NOT
+    assert grad(dy=None) == BAD and grad(x=P + 1) == BAD and grad(dx=P + 1) == BAD and grad(dtotal=P + 1) == BAD
+    assert grad(weight=P + 1) == BAD and grad(dweight=P + 1) == BAD and grad(eps=-1e-9) == BAD
+    need = K.reduce_norm_grad_workspace(4, 256)
+    assert need > 0 and grad(workspace=None) == BAD and grad(workspace_bytes=need - 1) == BAD and grad(workspace=P + 8) == BAD
+    rows = dict(dy=256, x=256, dtotal=256, dx=256)
+    for name in rows:
+        assert grad(strides={**rows, name: 255}) == BAD
+    assert grad(rows=1 << 31) == BAD
+    assert grad(dx=None, dweight=None, dy=None) == OK and grad(cols=0) == OK
+    assert grad(rows=0, dweight=None, dy=None, x=None) == OK
+    assert K.reduce_norm_grad_workspace(0, 256) == 0 and K.reduce_norm_grad_workspace(5, 0) == 0
+
+
+def product(**kw):
+    a = dict(y=P, x=P, w=P, offsets=P, experts=4, rows=64, n=128, k=256, dtype=N.DT_BF16)
+    a.update(kw)
+    return K.expert_product(**a)
+
+
+def test_product_refusals():
+    assert product(dtype=N.DT_FP32) == NOT and product(dtype=N.DT_E4M3) == NOT and product(dtype=10) == BAD
+    assert product(out_dtype=N.DT_FP16) == NOT and product(out_dtype=-1) == BAD and product(layout=2) == BAD
+    assert product(offsets=None) == BAD and product(offsets=P + 2) == BAD
+    assert product(y=None) == BAD and product(x=None) == BAD and product(w=P + 1) == BAD
+    assert product(y=P + 2, out_dtype=N.DT_FP32) == BAD
+    st = dict(x=256, w=256, y=128, expert_w=128 * 256)
+    for name, v in (("x", 255), ("w", 255), ("y", 127)):
+        assert product(strides={**st, name: v}) == BAD
+    assert product(layout=K.W_KN, strides={**st, "w": 127}) == BAD
+    assert product(rows=1 << 31) == BAD and product(n=1 << 31) == BAD and product(k=1 << 31) == BAD
+    assert product(rows=0, y=None, x=None) == OK and product(n=0, y=None) == OK and product(experts=0, y=None) == OK
+
+
+def test_product_dw_refusals():
+    def dw(**kw):
+        a = dict(dw=P, dy=P, x=P, offsets=P, experts=4, rows=64, n=128, k=256, dtype=N.DT_FP16)
+        a.update(kw)
+        return K.expert_product_dw(**a)
+    assert dw(dtype=N.DT_FP32) == NOT and dw(out_dtype=N.DT_BF16) == NOT and dw(dtype=12) == BAD
+    assert dw(offsets=None) == BAD and dw(dw=None) == BAD and dw(dy=None) == BAD and dw(x=P + 1) == BAD
+    st = dict(dy=128, x=256, dw=256, expert_dw=128 * 256)
+    for name, v in (("dy", 127), ("x", 255), ("dw", 255)):
+        assert dw(strides={**st, name: v}) == BAD
+    assert dw(rows=1 << 31) == BAD
+    assert dw(experts=0, dw=None) == OK and dw(n=0, dw=None) == OK and dw(k=0, dw=None) == OK
+
+
+def test_product_e4m3_refusals():
+    def e(**kw):
+        a = dict(y=P, x=P, xscale=P, w=P, wscale=P, offsets=P, experts=4, rows=64, n=128, k=300, out_dtype=N.DT_BF16)
+        a.update(kw)
+        return K.expert_product_e4m3(**a)
+    assert e(out_dtype=N.DT_E4M3) == NOT and e(out_dtype=N.DT_INT8) == NOT and e(out_dtype=50) == BAD
+    assert e(offsets=None) == BAD and e(y=P + 1) == BAD and e(x=None) == BAD and e(w=None) == BAD
+    assert e(xscale=None) == BAD and e(wscale=P + 2) == BAD
+    st = dict(x=300, w=300, y=128, expert_w=128 * 300, xscale=3, wscale=3, expert_wscale=3)
+    for name, v in (("x", 299), ("w", 299), ("y", 127), ("xscale", 2), ("wscale", 2)):
+        assert e(strides={**st, name: v}) == BAD
+    assert e(rows=0, y=None) == OK and e(n=0, y=None) == OK
+
+
+def test_norm_gradient_formula_against_differences():
+    rng = np.random.default_rng(5)
+    x, w, c, ct = (rng.standard_normal(s) for s in ((3, 17), (17,), (3, 17), (3, 17)))
+    eps = 1e-3
+    f = lambda x, w: float(np.sum(c * R.norm([x], None, w, eps)[1]) + np.sum(ct * x))  # noqa: E731
+    dx, dw, _, _ = R.norm_grad(c, x, w, ct, eps)
+    h = 1e-6
+    for r, q in ((0, 0), (1, 8), (2, 16)):
+        d = np.zeros_like(x)
+        d[r, q] = h
+        assert abs((f(x + d, w) - f(x - d, w)) / (2 * h) - dx[r, q]) < 1e-7
+    for q in (0, 9):
+        d = np.zeros_like(w)
+        d[q] = h
+        assert abs((f(x, w + d) - f(x, w - d)) / (2 * h) - dw[q]) < 1e-7
+
+
+def test_product_gradient_formula_against_differences():
+    rng = np.random.default_rng(6)
+    x, w, c, o = rng.standard_normal((7, 5)), rng.standard_normal((3, 4, 5)), rng.standard_normal((7, 4)), [0, 3, 3, 6]
+    f = lambda x, w: float(np.nansum(c * R.product(x, w, o, True)[0]))  # noqa: E731
+    dx, dw = R.product(c, w, o, False)[0], R.product_dw(c, x, o)[0]
+    h = 1e-6
+    for at in ((0, 1), (5, 4)):
+        d = np.zeros_like(x)
+        d[at] = h
+        assert abs((f(x + d, w) - f(x - d, w)) / (2 * h) - dx[at]) < 1e-7
+    for at in ((0, 0, 0), (1, 2, 2), (2, 3, 4)):
+        d = np.zeros_like(w)
+        d[at] = h
+        assert abs((f(x, w + d) - f(x, w - d)) / (2 * h) - dw[at]) < 1e-7
+    assert not dw[1].any() and np.isnan(dx[6]).all()
+
+
+def test_e4m3_table():
+    assert R.E4M3[0x7e] == 448 and R.E4M3[1] == 2.0 ** -9 and R.E4M3[0x38] == 1 and np.isnan(R.E4M3[0xff])
+    codes = np.array([c for c in range(256) if c & 127 != 127], np.uint8)
+    assert np.array_equal(R.to_e4m3(R.E4M3[codes]), codes)
+    assert R.to_e4m3(np.array([1.0625]))[0] == 0x38 and R.to_e4m3(np.array([1.1875]))[0] == 0x3a       # ties to even
+
+
+def test_header_is_plain_c(tmp_path):
+    if not shutil.which("gcc"):
+        pytest.skip("no gcc")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "client.c"
+    src.write_text(r'''
+#include <stddef.h>
+#include "flagcx_amd/fx_model.h"
+int main(void) {
+  size_t need = fx_reduce_norm_grad_workspace(3, 100);
+  if (need < 100 * sizeof(float)) return 1;
+  if (fx_reduce_norm(NULL, NULL, NULL, NULL, 1, NULL, NULL, 1, 1, NULL, flagcxBfloat16, flagcxBfloat16, flagcxBfloat16, 1e-6f, NULL) != flagcxInvalidArgument) return 2;
+  if (fx_expert_product(NULL, NULL, NULL, NULL, 1, 0, 8, 8, FX_WEIGHT_NK, NULL, flagcxFloat16, flagcxFloat32, NULL) != flagcxSuccess) return 3;
+  return 0;
+}
+''')
+    exe, libdir = tmp_path / "client", os.path.join(root, "flagcx_amd", "lib")
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Wextra", "-Werror", "-pedantic", f"-I{root}/include", str(src), "-o", str(exe),
+                    f"-L{libdir}", "-lflagcx-kernels-mi355x", f"-Wl,-rpath,{libdir}", "-Wl,-rpath,/opt/rocm/lib"], check=True)
+    subprocess.run([str(exe)], check=True)
+
+
+def test_stride_blocks_match_the_header():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = re.sub(r"/\*.*?\*/", "", open(os.path.join(root, "include", "flagcx_amd", "fx_model.h")).read(), flags=re.S)
+    for name, cls in (("fxNormStrides", N.NormStrides), ("fxNormGradStrides", N.NormGradStrides), ("fxProductStrides", N.ProductStrides),
+                      ("fxProductDwStrides", N.ProductDwStrides), ("fxProductE4m3Strides", N.ProductE4m3Strides)):
+        body = re.search(r"typedef struct %s \{(.*?)\}" % name, text, re.S).group(1)
+        fields = re.findall(r"\w+", body.replace("size_t", ""))
+        assert [f.rstrip("_") for f, _ in cls._fields_] == fields, name

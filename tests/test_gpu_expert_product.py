@@ -1,0 +1,300 @@
+"""Products grouped by expert against the 64-bit restatement."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from flagcx_amd import _native as N
+from flagcx_amd import kernels as K
+from tests import model_ref as R
+from tests.util import DevBufs
+
+pytestmark = pytest.mark.gpu
+
+NAN16 = {N.DT_BF16: 0x7fc0, N.DT_FP16: 0x7e00}
+
+
+def ragged(rows, experts, rng, empty=0.2):
+    """Ascending offsets with empty experts, a gap in front and one behind."""
+    inner = np.sort(rng.integers(0, rows + 1, experts + 1))
+    for e in range(1, experts + 1):
+        if rng.random() < empty:
+            inner[e] = inner[e - 1]
+    return inner.astype(np.int32)
+
+
+def with_ld(a, ld, fill):
+    out = np.full(a.shape[:-1] + (ld,), fill, a.dtype)
+    out[..., :a.shape[-1]] = a
+    return out
+
+
+def run(dev, dtype, rows, n, k, offsets, *, nk=True, out32=False, pad=0, shift=0, seed=0, stream=None):
+    experts = 1 if offsets is None else len(offsets) - 1
+    x, w = R.normal(dtype, (rows, k), seed), R.normal(dtype, (experts, n, k) if nk else (experts, k, n), seed + 1)
+    segs = offsets if offsets is not None else [0, rows]
+    inside = np.zeros(rows, bool)
+    for a, b in R.clamp_offsets(segs, rows):
+        inside[a:b] = True
+    x[~inside] = NAN16[dtype]                                # rows of nobody must not reach any result
+    odt = np.float32 if out32 else np.uint16
+    ldx, ldw, ldy = k + pad, w.shape[2] + pad, n + pad
+    st = dict(x=ldx, w=ldw, y=ldy, expert_w=w.shape[1] * ldw + pad) if pad else None
+    wbuf = with_ld(w, ldw, NAN16[dtype]).reshape(experts, -1)
+    if pad:
+        wbuf = np.concatenate([wbuf, np.full((experts, pad), NAN16[dtype], np.uint16)], axis=1)
+    fill = odt(9)
+    with DevBufs(dev) as b:
+        dx = b.put(with_ld(x, ldx, NAN16[dtype]), pad_before=2 * shift)
+        dw = b.put(wbuf, pad_before=2 * shift)
+        do = b.put(np.ascontiguousarray(offsets)) if offsets is not None else None
+        dy = b.put(np.full((rows, ldy), fill, odt), pad_before=shift * odt().itemsize)
+        N.check(K.expert_product(dy, dx, dw, do, experts, rows, n, k, dtype, out_dtype=N.DT_FP32 if out32 else None,
+                                 layout=K.W_NK if nk else K.W_KN, strides=st, stream=stream), "fx_expert_product")
+        dev.sync()
+        y = dev.to_host(dy, rows * ldy, odt).reshape(rows, ldy)
+    assert (y[:, n:] == fill).all() and (y[~inside] == fill).all(), "rows and columns of nobody stay as they were"
+    want, mag = R.product(R.codes_to_f64(x, dtype), R.codes_to_f64(w, dtype), segs, nk)
+    t = N.DT_FP32 if out32 else dtype
+    got = R.codes_to_f64(y[inside, :n], t)
+    want, mag = want[inside], mag[inside]
+    assert (np.abs(got - want) <= R.rounding(want, t) * 1.01 + R.sum_bound(k, mag)).all()
+    return y
+
+
+@pytest.mark.parametrize("name,dtype", [("bf16", N.DT_BF16), ("fp16", N.DT_FP16)])
+@pytest.mark.parametrize("nk", [True, False])
+@pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (3, 17, 5), (16, 64, 64), (17, 128, 72), (65, 100, 200), (130, 257, 136), (300, 520, 1000)])
+def test_plain_products(dev, name, dtype, nk, rows, n, k):
+    print(name, nk, rows, n, k, flush=True)
+    run(dev, dtype, rows, n, k, None, nk=nk, seed=rows)
+    run(dev, dtype, rows, n, k, None, nk=nk, out32=True, seed=rows)
+
+
+@pytest.mark.parametrize("nk", [True, False])
+@pytest.mark.parametrize("rows,experts,n,k", [(5, 3, 64, 64), (40, 8, 128, 256), (200, 5, 264, 328), (700, 13, 200, 96), (500, 70, 64, 128),
+                                              (90, 200, 32, 64), (1100, 3, 300, 520)])
+def test_ragged_products(dev, nk, rows, experts, n, k):
+    rng = np.random.default_rng(rows)
+    for dtype in (N.DT_BF16, N.DT_FP16):
+        o = ragged(rows, experts, rng)
+        print(nk, rows, experts, n, k, o.tolist()[:20], flush=True)
+        run(dev, dtype, rows, n, k, o, nk=nk, out32=dtype == N.DT_FP16, seed=rows)
+
+
+@pytest.mark.parametrize("nk", [True, False])
+def test_strides_and_alignment(dev, nk):
+    rng = np.random.default_rng(3)
+    for pad, shift in ((1, 0), (8, 0), (0, 1), (3, 1), (8, 4)):
+        for rows, n, k in ((50, 72, 136), (260, 136, 264), (33, 129, 65)):
+            print(nk, pad, shift, rows, n, k, flush=True)
+            run(dev, N.DT_BF16, rows, n, k, ragged(rows, 4, rng), nk=nk, pad=pad, shift=shift, seed=pad)
+
+
+def test_no_reduction_gives_zeros(dev):
+    with DevBufs(dev) as b:
+        y = b.put(np.full((5, 7), 3, np.uint16))
+        o = b.put(np.array([0, 2, 4], np.int32))
+        N.check(K.expert_product(y, None, None, o, 2, 5, 7, 0, N.DT_BF16))
+        dev.sync()
+        got = dev.to_host(y, 35, np.uint16).reshape(5, 7)
+    assert not got[:4].any() and (got[4] == 3).all()
+
+
+@pytest.mark.parametrize("offsets", [[-5, 3, 9, 400], [0, 30, 10, 40], [50, 40, 30, 20], [400, 400, 400, 400], [-9, -8, -7, -6]])
+def test_bad_offsets_touch_nothing_outside(dev, offsets):
+    """Clamped to the rows; a descending pair is an empty expert.  Rows claimed twice get either answer, so only the
+    guards around y and the finiteness of what lies inside are checked."""
+    rows, n, k = 40, 72, 64
+    x, w = R.normal(N.DT_BF16, (rows, k), 1), R.normal(N.DT_BF16, (3, n, k), 2)
+    guard = np.full((64, n), 9, np.uint16)
+    with DevBufs(dev) as b:
+        dx, dw, do = b.put(x), b.put(w), b.put(np.array(offsets, np.int32))
+        base = b.put(np.concatenate([guard, np.full((rows, n), 9, np.uint16), guard]))
+        dy, ddw = base + guard.nbytes, b.alloc(3 * n * k * 4)
+        N.check(K.expert_product(dy, dx, dw, do, 3, rows, n, k, N.DT_BF16))
+        N.check(K.expert_product_dw(ddw, dy, dx, do, 3, rows, n, k, N.DT_BF16, out_dtype=N.DT_FP32))
+        dev.sync()
+        y = dev.to_host(base, (rows + 128) * n, np.uint16).reshape(-1, n)
+        dwv = dev.to_host(ddw, 3 * n * k, np.float32)
+    assert (y[:64] == 9).all() and (y[-64:] == 9).all() and np.isfinite(dwv).all()
+
+
+def run_dw(dev, dtype, rows, n, k, offsets, *, out32=False, pad=0, shift=0, seed=0):
+    experts = 1 if offsets is None else len(offsets) - 1
+    dy, x = R.normal(dtype, (rows, n), seed), R.normal(dtype, (rows, k), seed + 1)
+    segs = offsets if offsets is not None else [0, rows]
+    inside = np.zeros(rows, bool)
+    for a, b in R.clamp_offsets(segs, rows):
+        inside[a:b] = True
+    dy[~inside] = NAN16[dtype]
+    x[~inside] = NAN16[dtype]
+    odt, t = (np.float32, N.DT_FP32) if out32 else (np.uint16, dtype)
+    fill = odt(9)
+    st = dict(dy=n + pad, x=k + pad, dw=k + pad, expert_dw=n * (k + pad) + pad) if pad else None
+    with DevBufs(dev) as b:
+        ddy = b.put(with_ld(dy, n + pad, NAN16[dtype]), pad_before=2 * shift)
+        dx = b.put(with_ld(x, k + pad, NAN16[dtype]), pad_before=2 * shift)
+        do = b.put(np.ascontiguousarray(offsets)) if offsets is not None else None
+        per = n * (k + pad) + pad
+        ddw = b.put(np.full(experts * per + 64, fill, odt), pad_before=shift * odt().itemsize)
+        N.check(K.expert_product_dw(ddw, ddy, dx, do, experts, rows, n, k, dtype, out_dtype=t, strides=st), "fx_expert_product_dw")
+        dev.sync()
+        dw = dev.to_host(ddw, experts * per + 64, odt)
+    assert (dw[experts * per:] == fill).all()
+    dw = dw[:experts * per].reshape(experts, per)
+    assert (dw[:, n * (k + pad):] == fill).all()
+    dw = dw[:, :n * (k + pad)].reshape(experts, n, k + pad)
+    assert (dw[:, :, k:] == fill).all()
+    want, mag = R.product_dw(R.codes_to_f64(dy, dtype), R.codes_to_f64(x, dtype), segs)
+    assert (np.abs(R.codes_to_f64(dw[:, :, :k], t) - want) <= R.rounding(want, t) * 1.01 + R.sum_bound(rows, mag)).all()
+
+
+@pytest.mark.parametrize("rows,experts,n,k", [(1, 1, 1, 1), (9, 2, 17, 5), (64, 1, 64, 64), (200, 5, 136, 264), (700, 13, 200, 96),
+                                              (90, 70, 32, 64), (1100, 3, 300, 520)])
+def test_weight_gradients(dev, rows, experts, n, k):
+    rng = np.random.default_rng(rows)
+    for dtype in (N.DT_BF16, N.DT_FP16):
+        o = ragged(rows, experts, rng)
+        print(dtype, rows, experts, n, k, o.tolist()[:20], flush=True)
+        run_dw(dev, dtype, rows, n, k, o, seed=rows)
+        run_dw(dev, dtype, rows, n, k, o, out32=True, seed=rows)
+    run_dw(dev, N.DT_BF16, rows, n, k, None, seed=rows)
+
+
+def test_weight_gradient_strides_and_alignment(dev):
+    rng = np.random.default_rng(3)
+    for pad, shift in ((1, 0), (8, 0), (0, 1), (3, 1), (8, 4)):
+        for rows, n, k in ((50, 72, 136), (260, 136, 264), (33, 129, 65)):
+            print(pad, shift, rows, n, k, flush=True)
+            run_dw(dev, N.DT_BF16, rows, n, k, ragged(rows, 4, rng), pad=pad, shift=shift, seed=pad)
+
+
+def test_weight_gradient_without_rows_is_zero(dev):
+    with DevBufs(dev) as b:
+        dw, o = b.put(np.full((2, 5, 7), 3, np.uint16)), b.put(np.zeros(3, np.int32))
+        N.check(K.expert_product_dw(dw, None, None, o, 2, 0, 5, 7, N.DT_BF16))
+        dev.sync()
+        assert not dev.to_host(dw, 70, np.uint16).any()
+
+
+# ------------------------------------------------------------------- e4m3
+
+def run8(dev, rows, n, k, offsets, out, *, pad=0, shift=0, seed=0, codes=None):
+    experts = 1 if offsets is None else len(offsets) - 1
+    rng = np.random.default_rng(seed)
+    kg, ng = -(-k // 128), -(-n // 128)
+    make = codes or (lambda s: R.to_e4m3(np.clip(rng.standard_normal(s) * 120, -448, 448)))
+    x, w = make((rows, k)), make((experts, n, k))
+    xs = np.exp2(rng.uniform(-9, 1, (rows, kg))).astype(np.float32)
+    ws = np.exp2(rng.uniform(-12, -4, (experts, ng, kg))).astype(np.float32)
+    segs = offsets if offsets is not None else [0, rows]
+    inside = np.zeros(rows, bool)
+    for a, b in R.clamp_offsets(segs, rows):
+        inside[a:b] = True
+    x[~inside] = 0x7f
+    xs[~inside] = np.nan
+    odt = np.float32 if out == N.DT_FP32 else np.uint16
+    fill = odt(9)
+    ldx, ldy = k + pad, n + pad
+    st = dict(x=ldx, w=ldx, y=ldy, expert_w=n * ldx + pad, xscale=kg + (pad > 0), wscale=kg + (pad > 0),
+              expert_wscale=ng * (kg + (pad > 0)) + pad) if pad else None
+    wbuf = with_ld(w, ldx, 0x7f).reshape(experts, -1)
+    wsbuf = with_ld(ws, kg + (pad > 0), np.nan).reshape(experts, -1)
+    if pad:
+        wbuf = np.concatenate([wbuf, np.full((experts, pad), 0x7f, np.uint8)], axis=1)
+        wsbuf = np.concatenate([wsbuf, np.full((experts, pad), np.nan, np.float32)], axis=1)
+    with DevBufs(dev) as b:
+        dx, dw = b.put(with_ld(x, ldx, 0x7f), pad_before=shift), b.put(wbuf, pad_before=shift)
+        dxs, dws = b.put(with_ld(xs, kg + (pad > 0), np.nan)), b.put(wsbuf)
+        do = b.put(np.ascontiguousarray(offsets)) if offsets is not None else None
+        dy = b.put(np.full((rows, ldy), fill, odt), pad_before=shift * odt().itemsize)
+        N.check(K.expert_product_e4m3(dy, dx, dxs, dw, dws, do, experts, rows, n, k, out, strides=st), "fx_expert_product_e4m3")
+        dev.sync()
+        y = dev.to_host(dy, rows * ldy, odt).reshape(rows, ldy)
+    assert (y[:, n:] == fill).all() and (y[~inside] == fill).all()
+    fx = R.E4M3[x] * np.repeat(xs.astype(np.float64), 128, axis=1)[:, :k]
+    fw = R.E4M3[w] * np.repeat(np.repeat(ws.astype(np.float64), 128, axis=2)[:, :, :k], 128, axis=1)[:, :n]
+    want, mag = R.product(fx, fw, segs, True)
+    want, mag = want[inside], mag[inside]
+    got = R.codes_to_f64(y[inside, :n], out)
+    # fp32 results: sums as in fp32.  16-bit ones: the 8-bit matrix instructions' own error per group of 128.
+    group = 0 if out == N.DT_FP32 else 2.0 ** -12
+    assert (np.abs(got - want) <= R.rounding(want, out) * 1.01 + R.sum_bound(min(k, 128) + kg + 4, mag) + group * mag).all()
+
+
+@pytest.mark.parametrize("out", [N.DT_BF16, N.DT_FP16, N.DT_FP32])
+@pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (3, 17, 5), (16, 64, 128), (17, 128, 144), (33, 500, 400), (65, 100, 200), (130, 257, 272),
+                                      (300, 520, 1000)])
+def test_e4m3_plain_products(dev, out, rows, n, k):
+    print(out, rows, n, k, flush=True)
+    run8(dev, rows, n, k, None, out, seed=rows)
+
+
+@pytest.mark.parametrize("rows,experts,n,k", [(5, 3, 64, 64), (40, 8, 128, 256), (200, 5, 264, 336), (700, 13, 200, 96), (90, 200, 32, 64),
+                                              (1100, 3, 300, 520)])
+def test_e4m3_ragged_products(dev, rows, experts, n, k):
+    rng = np.random.default_rng(rows)
+    for out in (N.DT_BF16, N.DT_FP32):
+        o = ragged(rows, experts, rng)
+        print(out, rows, experts, n, k, o.tolist()[:20], flush=True)
+        run8(dev, rows, n, k, o, out, seed=rows)
+
+
+def test_e4m3_strides_and_alignment(dev):
+    rng = np.random.default_rng(3)
+    for pad, shift in ((1, 0), (16, 0), (0, 1), (3, 1), (16, 16)):
+        for rows, n, k in ((50, 72, 144), (260, 136, 272), (33, 129, 65)):
+            print(pad, shift, rows, n, k, flush=True)
+            run8(dev, rows, n, k, ragged(rows, 4, rng), N.DT_BF16, pad=pad, shift=shift, seed=pad)
+            run8(dev, rows, n, k, ragged(rows, 4, rng), N.DT_FP32, pad=pad, shift=shift, seed=pad)
+
+
+# ------------------------------------------------------------------- graph
+
+hip = C.CDLL("libamdhip64.so.7")
+hip.hipStreamBeginCapture.argtypes = [C.c_void_p, C.c_int]
+hip.hipStreamEndCapture.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
+hip.hipGraphInstantiate.argtypes = [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
+hip.hipGraphLaunch.argtypes = [C.c_void_p, C.c_void_p]
+hip.hipGraphExecDestroy.argtypes = [C.c_void_p]
+hip.hipGraphDestroy.argtypes = [C.c_void_p]
+
+
+@pytest.mark.parametrize("rows,n,k", [(24, 96, 160), (600, 320, 512)])
+def test_products_replay_in_a_graph_with_new_routing(dev, rows, n, k):
+    """The captured calls read the offsets when they execute: every replay has other rows per expert."""
+    experts, t = 6, N.DT_BF16
+    stream = dev.stream_create()
+    raw = dev.raw_stream(stream)
+    rng = np.random.default_rng(1)
+    with DevBufs(dev) as b:
+        w = R.normal(t, (experts, n, k), 9)
+        dw, dx, do = b.put(w), b.alloc(rows * k * 2), b.alloc(64)
+        dy, dg = b.alloc(rows * n * 2), b.alloc(experts * n * k * 4)
+        graph, gexec = C.c_void_p(), C.c_void_p()
+        assert hip.hipStreamBeginCapture(raw, 0) == 0
+        try:
+            N.check(K.expert_product(dy, dx, dw, do, experts, rows, n, k, t, stream=raw))
+            N.check(K.expert_product_dw(dg, dy, dx, do, experts, rows, n, k, t, out_dtype=N.DT_FP32, stream=raw))
+        finally:
+            assert hip.hipStreamEndCapture(raw, C.byref(graph)) == 0
+        assert hip.hipGraphInstantiate(C.byref(gexec), graph, None, None, 0) == 0
+        for rep in range(4):
+            o = ragged(rows, experts, rng)
+            dev.upload(dx, R.normal(t, (rows, k), rep))
+            dev.upload(do, o)
+            dev.memset(dy, 0, rows * n * 2)
+            dev.sync()
+            assert hip.hipGraphLaunch(gexec, raw) == 0
+            dev.stream_sync(stream)
+            got = dev.to_host(dy, rows * n, np.uint16), dev.to_host(dg, experts * n * k, np.uint32)
+            dev.memset(dy, 0, rows * n * 2)
+            N.check(K.expert_product(dy, dx, dw, do, experts, rows, n, k, t))
+            N.check(K.expert_product_dw(dg, dy, dx, do, experts, rows, n, k, t, out_dtype=N.DT_FP32))
+            dev.sync()
+            assert np.array_equal(got[0], dev.to_host(dy, rows * n, np.uint16))
+            assert np.array_equal(got[1], dev.to_host(dg, experts * n * k, np.uint32))
+        hip.hipGraphExecDestroy(gexec)
+        hip.hipGraphDestroy(graph)
+    dev.stream_destroy(stream)
