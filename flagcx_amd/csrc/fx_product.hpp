@@ -448,6 +448,93 @@ __global__ void __launch_bounds__(WN *WM * 64) productGuarded(ProductArgs a) {
   p.store(a, t);
 }
 
+// Aligned operands: the chunks go from memory to LDS without passing through
+// registers (buffer loads with the LDS flag), one slab ahead, into the other of
+// two buffers.  A wavefront's 64 chunks land in 1024 consecutive bytes, so the
+// exchange of chunks is in the addresses that the lanes load from.  Chunks that
+// do not exist are given an offset outside the buffer and arrive as zeros.
+//
+// The loads are issued from inline assembly (they have no register outputs): the
+// compiler does not know that they write LDS, and every read of LDS behind one
+// would otherwise wait for it.  The waits are therefore written here: a slab is
+// read only behind a wait for all of this wavefront's loads and a barrier.
+constexpr uint32_t kOutside = 0x80000000u;
+__device__ __forceinline__ void loadToLds(uint32_t ldsAt, uint32_t voff, __amdgpu_buffer_rsrc_t rsrc, uint32_t soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(ldsAt), "v"(voff), "s"(rsrc), "s"(soff));
+}
+__device__ __forceinline__ void waitAndMeet() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <int R, int NT, int ES, bool ACROSS, bool NSIDE>
+struct DirectSide : Side<R, NT, ES, ACROSS, NSIDE> {
+  using S = Side<R, NT, ES, ACROSS, NSIDE>;
+  uint32_t voff[S::kLoads];
+  uint32_t step;          // bytes between a thread's chunks
+  uint64_t at, advance;   // address of the slab to load next; bytes per slab
+  __device__ __forceinline__ void start(const char *base, size_t ld, uint32_t own) {
+    S::init();
+    step = uniform((uint32_t)(S::kStep * ld * ES));
+    at = (uint64_t)(uintptr_t)base;
+    advance = ACROSS ? S::kSlab * ld * ES : 128;
+    const uint32_t off = (uint32_t)((S::row * ld + S::chunk * S::kElems) * ES);
+#pragma unroll
+    for (int q = 0; q < S::kLoads; q++)
+      voff[q] = (ACROSS ? S::chunk * S::kElems < own : S::row + q * S::kStep < own) ? off : kOutside;
+  }
+  // red: reduction elements left from this slab on
+  __device__ __forceinline__ void issue(uint32_t lds, uint32_t wave, uint32_t red) {
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)at, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+    for (int q = 0; q < S::kLoads; q++) {
+      const bool there = ACROSS ? S::row + q * S::kStep < red : S::chunk * S::kElems < red;
+      loadToLds(lds + (q * NT + wave * 64) * 16, there ? voff[q] : kOutside, rsrc, q * step);
+    }
+    at += advance;
+  }
+};
+
+template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW>
+__global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
+  using P = Product<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>;
+  constexpr uint32_t kStage = P::kLdsN + P::kLdsM;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+  typedef __attribute__((address_space(3))) char *ldsPtr;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(ldsPtr)lds;
+  Tile t;
+  if (!(DW ? findTileDw<BN, BM>(a, &t) : findTile<BN, BM>(a, &t))) return;
+  P p;
+  p.init();
+  const uint32_t wave = uniform(threadIdx.x >> 6);
+  DirectSide<BN, P::kThreads, P::ES, NACROSS, true> sn;
+  DirectSide<BM, P::kThreads, P::ES, MACROSS, false> sm;
+  const size_t nAt = NACROSS ? (size_t)t.k0 * a.ldn + t.n0 : (size_t)t.n0 * a.ldn + t.k0;
+  const size_t mAt = MACROSS ? (size_t)t.k0 * a.ldm + t.m0 : (size_t)t.m0 * a.ldm + t.k0;
+  sn.start((const char *)a.pn + (nAt + (DW ? 0 : (size_t)t.expert * a.expertN)) * P::ES, a.ldn, a.n - t.n0);
+  sm.start((const char *)a.pm + mAt * P::ES, a.ldm, t.mEnd - t.m0);
+  const uint32_t slabs = (t.kLen + P::kSlab - 1) / P::kSlab;
+  uint32_t red = t.kLen;
+  float scale[P::FM], next[P::FM];
+  auto issue = [&](uint32_t s) {
+    const uint32_t at = lds0 + (s & 1) * kStage;
+    sn.issue(at, wave, red);
+    sm.issue(at + P::kLdsN, wave, red);
+    red -= P::kSlab;
+    p.scales(a, t, s, next);
+  };
+  if (slabs) issue(0);
+  for (uint32_t s = 0; s < slabs; s++) {
+    waitAndMeet();
+#pragma unroll
+    for (int q = 0; q < P::FM; q++) scale[q] = next[q];
+    if (s + 1 < slabs) issue(s + 1);
+    p.slab(lds + (s & 1) * kStage, lds + (s & 1) * kStage + P::kLdsN, scale);
+  }
+  p.store(a, t);
+}
+
 // ------------------------------------------------------------- launch tables
 
 enum ProductForm { kFormNK = 0, kFormKN = 1, kFormDw = 2 };
@@ -457,8 +544,8 @@ flagcxResult_t launchProductBf16(const ProductArgs &a, int form, bool outF32, hi
 flagcxResult_t launchProductF16(const ProductArgs &a, int form, bool outF32, hipStream_t s);
 flagcxResult_t launchProductE4m3(const ProductArgs &a, int outDtype, hipStream_t s);
 
-template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW>
-flagcxResult_t launchGuarded(ProductArgs a, hipStream_t s) {
+template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW, bool DIRECT>
+flagcxResult_t launchTiles(ProductArgs a, hipStream_t s) {
   a.nTiles = (a.n + BN - 1) / BN;
   if (DW) a.mTiles = (a.m + BM - 1) / BM;
   else if (!a.offsets) a.mTiles = (a.rows + BM - 1) / BM;
@@ -466,17 +553,39 @@ flagcxResult_t launchGuarded(ProductArgs a, hipStream_t s) {
   const uint64_t grid = (uint64_t)a.nTiles * a.mTiles * (DW ? a.experts : 1);
   if (grid > 0x7fffffffu) return flagcxNotSupported;
   void *argv[] = {&a};
-  const void *kernel = reinterpret_cast<const void *>(productGuarded<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
+  const void *kernel;
+  if constexpr (DIRECT) kernel = reinterpret_cast<const void *>(productDirect<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
+  else kernel = reinterpret_cast<const void *>(productGuarded<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
   return hipLaunchKernel(kernel, dim3((uint32_t)grid), dim3(WN * WM * 64), argv, 0, s) == hipSuccess ? flagcxSuccess
                                                                                                    : flagcxUnhandledDeviceError;
+}
+
+// Whole 16-byte chunks everywhere: what the direct kernels assume.  `inner` is the
+// contiguous extent of the operand's rows.
+inline bool wholeChunks(const void *p, size_t ld, size_t expert, size_t inner, size_t es) {
+  const size_t e = 16 / es;
+  return ((uintptr_t)p & 15) == 0 && ld % e == 0 && expert % e == 0 && inner % e == 0 && ld * es < (1u << 22);
+}
+
+template <class T, class Out, bool NACROSS, bool MACROSS, bool DW>
+flagcxResult_t launchShapes(const ProductArgs &a, hipStream_t s) {
+  const size_t es = kBytes<T>;
+  const bool direct = wholeChunks(a.pn, a.ldn, a.expertN, NACROSS ? a.n : a.k, es) &&
+                      wholeChunks(a.pm, a.ldm, 0, MACROSS ? a.m : a.k, es);
+  if (!direct) return launchTiles<T, Out, 128, 128, 2, 2, NACROSS, MACROSS, DW, false>(a, s);
+  // Tiles of 256 x 256 when they fill the 256 compute units, else of 128 x 128.
+  const uint64_t big = DW ? (uint64_t)a.experts * ((a.m + 255) / 256) * ((a.n + 255) / 256)
+                          : ((uint64_t)a.rows / 256 + a.experts / 2) * ((a.n + 255) / 256);
+  if (big >= 192) return launchTiles<T, Out, 256, 256, 4, 2, NACROSS, MACROSS, DW, true>(a, s);
+  return launchTiles<T, Out, 128, 128, 2, 2, NACROSS, MACROSS, DW, true>(a, s);
 }
 
 template <class T, class Out>
 flagcxResult_t launchForm(const ProductArgs &a, int form, hipStream_t s) {
   switch (form) {
-    case kFormNK: return launchGuarded<T, Out, 128, 128, 2, 2, false, false, false>(a, s);
-    case kFormKN: return launchGuarded<T, Out, 128, 128, 2, 2, true, false, false>(a, s);
-    default: return launchGuarded<T, Out, 128, 128, 2, 2, true, true, true>(a, s);
+    case kFormNK: return launchShapes<T, Out, false, false, false>(a, s);
+    case kFormKN: return launchShapes<T, Out, true, false, false>(a, s);
+    default: return launchShapes<T, Out, true, true, true>(a, s);
   }
 }
 

@@ -2,9 +2,9 @@
 namespace fx {
 flagcxResult_t launchProductE4m3(const ProductArgs &a, int outDtype, hipStream_t s) {
   switch (outDtype) {
-    case flagcxBfloat16: return launchForm<E4m3, __bf16>(a, kFormNK, s);
-    case flagcxFloat16: return launchForm<E4m3, _Float16>(a, kFormNK, s);
-    default: return launchForm<E4m3Exact, float>(a, kFormNK, s);
+    case flagcxBfloat16: return launchShapes<E4m3, __bf16, false, false, false>(a, s);
+    case flagcxFloat16: return launchShapes<E4m3, _Float16, false, false, false>(a, s);
+    default: return launchShapes<E4m3Exact, float, false, false, false>(a, s);
   }
 }
 }  // namespace fx

@@ -119,3 +119,12 @@ def product_dw(dy, x, offsets):
 def sum_bound(terms, mag):
     """A chain of `terms` fp32 additions in any order; the matrix cores may truncate where a sum would round."""
     return (terms + 8) * 2 * E * mag
+
+
+def within(got, want, t, bound):
+    """got is want, off by `bound` at most, rounded to type t.  fp16 ends at 65504: what rounds to 65520 or more is an
+    infinity of want's sign."""
+    fine = np.abs(got - want) <= rounding(want, t) * 1.01 + bound
+    if t == N.DT_FP16:
+        fine |= (np.abs(want) + bound >= 65520) & (got == np.copysign(np.inf, want))
+    return bool(fine.all())

@@ -91,6 +91,17 @@ def test_strides_and_alignment(dev, nk):
             run(dev, N.DT_BF16, rows, n, k, ragged(rows, 4, rng), nk=nk, pad=pad, shift=shift, seed=pad)
 
 
+@pytest.mark.parametrize("nk", [True, False])
+def test_large_products(dev, nk):
+    """Sizes that fill the chip: aligned operands (with an odd tail of the reduction, ragged rows and a partial last
+    column tile) and unaligned ones."""
+    rng = np.random.default_rng(8)
+    for rows, experts, n, k, pad in ((3200, 1, 4160, 200, 0), (3300, 7, 4168, 136, 8), (3100, 40, 4104, 64, 0), (3300, 7, 4168, 136, 1)):
+        o = None if experts == 1 else ragged(rows, experts, rng)
+        print(nk, rows, experts, n, k, pad, flush=True)
+        run(dev, N.DT_BF16, rows, n, k, o, nk=nk, pad=pad, seed=k, out32=pad == 8)
+
+
 def test_no_reduction_gives_zeros(dev):
     with DevBufs(dev) as b:
         y = b.put(np.full((5, 7), 3, np.uint16))
@@ -170,6 +181,13 @@ def test_weight_gradient_strides_and_alignment(dev):
             run_dw(dev, N.DT_BF16, rows, n, k, ragged(rows, 4, rng), pad=pad, shift=shift, seed=pad)
 
 
+def test_large_weight_gradients(dev):
+    rng = np.random.default_rng(8)
+    for rows, experts, n, k, pad in ((300, 1, 4104, 4096, 0), (500, 4, 2080, 2056, 8), (200, 4, 2080, 2056, 1)):
+        print(rows, experts, n, k, pad, flush=True)
+        run_dw(dev, N.DT_FP16, rows, n, k, None if experts == 1 else ragged(rows, experts, rng), pad=pad, seed=k, out32=pad == 8)
+
+
 def test_weight_gradient_without_rows_is_zero(dev):
     with DevBufs(dev) as b:
         dw, o = b.put(np.full((2, 5, 7), 3, np.uint16)), b.put(np.zeros(3, np.int32))
@@ -220,7 +238,7 @@ def run8(dev, rows, n, k, offsets, out, *, pad=0, shift=0, seed=0, codes=None):
     got = R.codes_to_f64(y[inside, :n], out)
     # fp32 results: sums as in fp32.  16-bit ones: the 8-bit matrix instructions' own error per group of 128.
     group = 0 if out == N.DT_FP32 else 2.0 ** -12
-    assert (np.abs(got - want) <= R.rounding(want, out) * 1.01 + R.sum_bound(min(k, 128) + kg + 4, mag) + group * mag).all()
+    assert R.within(got, want, out, R.sum_bound(min(k, 128) + kg + 4, mag) + group * mag)
 
 
 @pytest.mark.parametrize("out", [N.DT_BF16, N.DT_FP16, N.DT_FP32])
@@ -248,6 +266,15 @@ def test_e4m3_strides_and_alignment(dev):
             print(pad, shift, rows, n, k, flush=True)
             run8(dev, rows, n, k, ragged(rows, 4, rng), N.DT_BF16, pad=pad, shift=shift, seed=pad)
             run8(dev, rows, n, k, ragged(rows, 4, rng), N.DT_FP32, pad=pad, shift=shift, seed=pad)
+
+
+@pytest.mark.parametrize("out", [N.DT_BF16, N.DT_FP16, N.DT_FP32])
+def test_e4m3_large_products(dev, out):
+    rng = np.random.default_rng(8)
+    for rows, experts, n, k, pad in ((3200, 1, 4160, 400, 0), (3300, 7, 4176, 272, 16), (3100, 40, 4112, 128, 0), (3300, 7, 4176, 272, 1)):
+        o = None if experts == 1 else ragged(rows, experts, rng)
+        print(out, rows, experts, n, k, pad, flush=True)
+        run8(dev, rows, n, k, o, out, pad=pad, seed=k)
 
 
 # ------------------------------------------------------------------- graph
