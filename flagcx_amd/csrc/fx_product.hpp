@@ -496,10 +496,46 @@ struct DirectSide : Side<R, NT, ES, ACROSS, NSIDE> {
   }
 };
 
+// The e4m3 rows' scales of one slab, one float per row of the tile, brought to LDS
+// in the order in which a lane wants them (its fragments' rows side by side).
+template <int BM, int TM>
+struct DirectScales {
+  static constexpr uint32_t FM = TM / 16;
+  uint32_t voff;
+  uint64_t at;
+  __device__ __forceinline__ void start(const float *base, size_t ld, uint32_t own) {
+    const uint32_t pos = threadIdx.x, rem = pos % TM, row = pos / TM * TM + 16 * (rem % FM) + rem / FM;
+    voff = pos < BM && row < own ? (uint32_t)(row * ld * 4) : kOutside;
+    at = (uint64_t)(uintptr_t)base;
+  }
+  __device__ __forceinline__ void issue(uint32_t lds, uint32_t wave, bool there) {
+    if (wave * 64 < BM) {
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)at, 0, 0x7fffffff, 0x00020000);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds + wave * 256),
+                   "v"(there ? voff : kOutside), "s"(rsrc));
+    }
+    at += 4;
+  }
+};
+
+// The slabs as a pipeline.  A slab is multiplied in phases; the fragments of
+// the next phase are read from LDS while this one's are multiplied.  In front of
+// the last phase all of a slab's fragments are in registers: there the wavefronts
+// meet, its buffer is handed to the loads of the slab after the next, and the next
+// slab, whose loads have had a whole slab's time, is read from.  Loads past the
+// last slab have no lanes inside the buffer and read nothing.
+//
+// 16 bits: two halves of the reduction, each with two groups of m fragments.
+// e4m3: a phase is one m fragment (registers: 128 of accumulators, 32 of n
+// fragments); a product of 128 goes to registers of its own and is scaled into the
+// accumulators two products later, in the shadow of the matrix instructions.
+#define FX_FENCE() __builtin_amdgcn_sched_barrier(0)
+
 template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW>
 __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
   using P = Product<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>;
-  constexpr uint32_t kStage = P::kLdsN + P::kLdsM;
+  constexpr uint32_t kScales = P::kScaled ? 1024 : 0, kStage = P::kLdsN + P::kLdsM + kScales;
+  static_assert(BM <= 256, "room for the scales");
   __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
   typedef __attribute__((address_space(3))) char *ldsPtr;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(ldsPtr)lds;
@@ -507,31 +543,134 @@ __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
   if (!(DW ? findTileDw<BN, BM>(a, &t) : findTile<BN, BM>(a, &t))) return;
   P p;
   p.init();
-  const uint32_t wave = uniform(threadIdx.x >> 6);
+  const uint32_t wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   DirectSide<BN, P::kThreads, P::ES, NACROSS, true> sn;
   DirectSide<BM, P::kThreads, P::ES, MACROSS, false> sm;
+  DirectScales<BM, P::TM> ss;
   const size_t nAt = NACROSS ? (size_t)t.k0 * a.ldn + t.n0 : (size_t)t.n0 * a.ldn + t.k0;
   const size_t mAt = MACROSS ? (size_t)t.k0 * a.ldm + t.m0 : (size_t)t.m0 * a.ldm + t.k0;
   sn.start((const char *)a.pn + (nAt + (DW ? 0 : (size_t)t.expert * a.expertN)) * P::ES, a.ldn, a.n - t.n0);
   sm.start((const char *)a.pm + mAt * P::ES, a.ldm, t.mEnd - t.m0);
+  const float *blockScale = nullptr;
+  if constexpr (P::kScaled) {
+    ss.start(a.sm + (size_t)t.m0 * a.ldsm, a.ldsm, t.mEnd - t.m0);
+    const uint32_t last = (a.n - 1) / FX_SCALE_GROUP, b = (t.n0 + p.wn) / FX_SCALE_GROUP;
+    blockScale = a.sn + (size_t)t.expert * a.expertSn + (size_t)(b < last ? b : last) * a.ldsn;
+  }
   const uint32_t slabs = (t.kLen + P::kSlab - 1) / P::kSlab;
   uint32_t red = t.kLen;
-  float scale[P::FM], next[P::FM];
   auto issue = [&](uint32_t s) {
     const uint32_t at = lds0 + (s & 1) * kStage;
     sn.issue(at, wave, red);
     sm.issue(at + P::kLdsN, wave, red);
-    red -= P::kSlab;
-    p.scales(a, t, s, next);
+    if constexpr (P::kScaled) ss.issue(at + P::kLdsN + P::kLdsM, wave, red != 0);
+    red = red > P::kSlab ? red - P::kSlab : 0;
   };
-  if (slabs) issue(0);
-  for (uint32_t s = 0; s < slabs; s++) {
+  if (slabs) {
+    issue(0);
     waitAndMeet();
+    issue(1);
+    if constexpr (P::kScaled) {
+      u32x4 n[P::FN][2], m[2][2];
+      f32x4 part[3];
+      float scale[2];
+      uint32_t cur = 0;
+      float blocks = 0.f;                     // lane l: the block's scale of slab 64 * (s / 64) + l
+      const char *ln = lds, *lm = lds + P::kLdsN;
+      auto readM = [&](int q) {
+        const int fragment = q % P::FM;
+        m[q & 1][0] = p.readM(lm, fragment, 0);
+        m[q & 1][1] = p.readM(lm, fragment, 1);
+        scale[q & 1] = *reinterpret_cast<const float *>(lm + P::kLdsM + (p.wm + p.i * P::FM + fragment) * 4);
+      };
+      auto readN = [&](int f) {
+        n[f][0] = p.readN(ln, f, 0);
+        n[f][1] = p.readN(ln, f, 1);
+      };
+      readM(0);
 #pragma unroll
-    for (int q = 0; q < P::FM; q++) scale[q] = next[q];
-    if (s + 1 < slabs) issue(s + 1);
-    p.slab(lds + (s & 1) * kStage, lds + (s & 1) * kStage + P::kLdsN, scale);
+      for (int f = 0; f < P::FN; f++) readN(f);
+      for (uint32_t s = 0; s < slabs; s++) {
+        if ((s & 63) == 0) blocks = s + lane < slabs ? blockScale[s + lane] : 0.f;
+        const float sb = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, blocks), (int)(s & 63)));
+        float w[P::FM];
+        auto scaled = [&](int at) {           // product `at` into its accumulators
+          const int f = at % P::FN, q = at / P::FN;
+#pragma unroll
+          for (int v = 0; v < 4; v++) p.acc[f][q][v] = __builtin_fmaf(part[at % 3][v], w[q], p.acc[f][q][v]);
+          asm volatile("" : "+v"(p.acc[f][q]));   // here, not sunk behind the slab with all products alive
+        };
+#pragma unroll
+        for (int q = 0; q < P::FM; q++) {
+          if (q == P::FM - 1) {
+            FX_FENCE();
+            waitAndMeet();
+            issue(s + 2);
+            cur ^= kStage;                    // kStage or 0
+            ln = lds + cur;
+            lm = ln + P::kLdsN;
+          }
+          FX_FENCE();
+          w[q] = scale[q & 1] * sb;
+          readM(q + 1);                       // FM is even: FM is fragment 0 of the next slab, in buffer 0
+          FX_FENCE();
+#pragma unroll
+          for (int f = 0; f < P::FN; f++) {
+            const int at = q * P::FN + f;
+            part[at % 3] = mma8<T>(n[f], m[q & 1]);
+            if (at >= 2) scaled(at - 2);
+            FX_FENCE();
+            if (q == P::FM - 1) readN(f);
+          }
+        }
+        scaled(P::FM * P::FN - 2);
+        scaled(P::FM * P::FN - 1);
+      }
+    } else {
+      constexpr int GQ = P::FM / 2;
+      u32x4 n[2][P::FN], m[2][GQ];
+      uint32_t cur = 0;
+      const char *ln = lds, *lm = lds + P::kLdsN;
+      auto readN = [&](int half) {
+#pragma unroll
+        for (int f = 0; f < P::FN; f++) n[half][f] = p.readN(ln, f, half);
+      };
+      auto readM = [&](int ph) {
+#pragma unroll
+        for (int j = 0; j < GQ; j++) m[ph & 1][j] = p.readM(lm, (ph & 1) * GQ + j, ph >> 1);
+      };
+      readN(0);
+      readM(0);
+      for (uint32_t s = 0; s < slabs; s++) {
+#pragma unroll
+        for (int ph = 0; ph < 4; ph++) {
+          if (ph == 3) {
+            FX_FENCE();
+            waitAndMeet();
+            issue(s + 2);
+            cur ^= kStage;
+            ln = lds + cur;
+            lm = ln + P::kLdsN;
+          }
+          FX_FENCE();
+          readM((ph + 1) & 3);
+          if (ph == 0) readN(1);
+          if (ph == 3) readN(0);
+          FX_FENCE();
+#pragma unroll
+          for (int j = 0; j < GQ; j++)
+#pragma unroll
+            for (int f = 0; f < P::FN; f++) {
+              const int q = (ph & 1) * GQ + j;
+              p.acc[f][q] = mma<T>(n[ph >> 1][f], m[ph & 1][j], p.acc[f][q]);
+            }
+          FX_FENCE();
+        }
+      }
+    }
   }
+  // The loads behind the last slab have to have ended before this workgroup's LDS is another's.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   p.store(a, t);
 }
 
@@ -576,7 +715,8 @@ flagcxResult_t launchShapes(const ProductArgs &a, hipStream_t s) {
   // Tiles of 256 x 256 when they fill the 256 compute units, else of 128 x 128.
   const uint64_t big = DW ? (uint64_t)a.experts * ((a.m + 255) / 256) * ((a.n + 255) / 256)
                           : ((uint64_t)a.rows / 256 + a.experts / 2) * ((a.n + 255) / 256);
-  if (big >= 192) return launchTiles<T, Out, 256, 256, 4, 2, NACROSS, MACROSS, DW, true>(a, s);
+  if constexpr (!__is_same(T, E4m3Exact))      // widened operands leave no registers for the large tile
+    if (big >= 192) return launchTiles<T, Out, 256, 256, 4, 2, NACROSS, MACROSS, DW, true>(a, s);
   return launchTiles<T, Out, 128, 128, 2, 2, NACROSS, MACROSS, DW, true>(a, s);
 }
 
