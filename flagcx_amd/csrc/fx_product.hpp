@@ -140,10 +140,10 @@ __device__ __forceinline__ bool findTile(const ProductArgs &a, Tile *t) {
 
 template <int BN, int BM>
 __device__ __forceinline__ bool findTileDw(const ProductArgs &a, Tile *t) {
-  const uint32_t per = a.mTiles * a.nTiles;
-  const uint32_t id = dieOrder(blockIdx.x, per * a.experts), e = id / per;
+  // Experts differ in length, so each one's tiles are dealt to all dies.
+  const uint32_t per = a.mTiles * a.nTiles, e = blockIdx.x / per;
   uint32_t mt, nt, first = 0, last = a.rows;
-  panelOrder(id - e * per, a.mTiles, a.nTiles, &mt, &nt);
+  panelOrder(dieOrder(blockIdx.x - e * per, per), a.mTiles, a.nTiles, &mt, &nt);
   if (a.offsets) {
     first = uniform(bound(a, e));
     last = uniform(bound(a, e + 1));
@@ -674,6 +674,140 @@ __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
   p.store(a, t);
 }
 
+// Few rows per expert: the weights are read once, straight into registers, and
+// memory bounds the call.  A workgroup owns 16 RN columns of the output and up to
+// 16 FM rows; its wavefronts share the reduction, slab by slab in turn (so that
+// together they read long runs of each weight row), and their partial sums meet
+// in LDS in a fixed order.  Fragments without a row are skipped.  U slabs are
+// loaded while U are multiplied.  e4m3 operands are widened to bf16, whose sums are
+// those of fp32: the matrix cores have time.
+template <class T, class Out, int RN, int FM, int NW, int U>
+__global__ void __launch_bounds__(NW * 64) productThin(ProductArgs a) {
+  constexpr int BN = 16 * RN, BM = 16 * FM, ES = kBytes<T>, kElems = 16 / ES;
+  constexpr bool kScaled = ES == 1;
+  constexpr uint32_t kSlab = 128 / ES;
+  __shared__ f32x4 lds[NW][RN * FM][64];
+  Tile t;
+  if (!findTile<BN, BM>(a, &t)) return;
+  const uint32_t wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const uint32_t own = t.mEnd - t.m0, live = own >= (uint32_t)BM ? FM : (own + 15) / 16;
+  const uint32_t slabs = (a.k + kSlab - 1) / kSlab;
+  const char *pw[RN], *px[FM];
+  bool xHere[FM];
+#pragma unroll
+  for (int r = 0; r < RN; r++) {
+    const uint32_t n = t.n0 + 16 * r + i;      // columns behind the last repeat it; they are not stored
+    pw[r] = (const char *)a.pn + ((size_t)t.expert * a.expertN + (size_t)(n < a.n ? n : a.n - 1) * a.ldn) * ES;
+  }
+#pragma unroll
+  for (int f = 0; f < FM; f++) {
+    xHere[f] = 16 * f + i < own;
+    px[f] = (const char *)a.pm + (size_t)(t.m0 + 16 * f + (xHere[f] ? i : 0)) * a.ldm * ES;
+  }
+  const float *ps = nullptr, *pb = nullptr;
+  if constexpr (kScaled) {
+    ps = a.sm + (size_t)t.m0 * a.ldsm;
+    pb = a.sn + (size_t)t.expert * a.expertSn;
+  }
+  f32x4 acc[RN][FM];
+#pragma unroll
+  for (int r = 0; r < RN; r++)
+#pragma unroll
+    for (int f = 0; f < FM; f++) acc[r][f] = f32x4{};
+
+  struct Batch {
+    u32x4 w[U][RN][2], x[U][FM][2];
+    float sx[U][FM], sb[U][RN];
+  };
+  auto chunk = [&](const char *p, uint32_t c, bool tail) -> u32x4 {
+    if (!tail || (c + 1) * kElems <= a.k) return *reinterpret_cast<const u32x4_anywhere *>(p + c * 16);
+    u32x4 v = {};
+#pragma unroll
+    for (int j = 0; j < kElems; j++)
+      if (c * kElems + j < a.k) {
+        if constexpr (ES == 2) v[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[c * kElems + j] << (16 * (j & 1));
+        else v[j >> 2] |= (uint32_t)reinterpret_cast<const uint8_t *>(p)[c * kElems + j] << (8 * (j & 3));
+      }
+    return v;
+  };
+  // slabs s, s + NW, ...; the reduction's last slab may be partial
+  auto load = [&](Batch &b, uint32_t s0) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint32_t s = s0 + u * NW;
+      if (s >= slabs) continue;
+      const bool tail = (s + 1) * kSlab > a.k;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint32_t c = s * 8 + h * 4 + g;
+#pragma unroll
+        for (int r = 0; r < RN; r++) b.w[u][r][h] = chunk(pw[r], c, tail);
+#pragma unroll
+        for (int f = 0; f < FM; f++)
+          if (f == 0 || (uint32_t)f < live) {
+            b.x[u][f][h] = u32x4{};
+            if (xHere[f]) b.x[u][f][h] = chunk(px[f], c, tail);
+          }
+      }
+      if constexpr (kScaled) {
+#pragma unroll
+        for (int f = 0; f < FM; f++)
+          if (f == 0 || (uint32_t)f < live) b.sx[u][f] = xHere[f] ? ps[(size_t)(16 * f + i) * a.ldsm + s] : 0.f;
+#pragma unroll
+        for (int r = 0; r < RN; r++) b.sb[u][r] = pb[(size_t)((t.n0 + 16 * r < a.n ? t.n0 + 16 * r : a.n - 1) / FX_SCALE_GROUP) * a.ldsn + s];
+      }
+    }
+  };
+  auto multiply = [&](const Batch &b, uint32_t s0) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (s0 + u * NW >= slabs) continue;
+#pragma unroll
+      for (int f = 0; f < FM; f++)
+        if (f == 0 || (uint32_t)f < live)
+#pragma unroll
+          for (int r = 0; r < RN; r++) {
+            if constexpr (kScaled) {
+              const f32x4 p = mma8<E4m3Exact>(b.w[u][r], b.x[u][f]);
+              const float sc = b.sx[u][f] * b.sb[u][r];
+#pragma unroll
+              for (int v = 0; v < 4; v++) acc[r][f][v] = __builtin_fmaf(p[v], sc, acc[r][f][v]);
+            } else {
+#pragma unroll
+              for (int h = 0; h < 2; h++) acc[r][f] = mma<T>(b.w[u][r][h], b.x[u][f][h], acc[r][f]);
+            }
+          }
+    }
+  };
+  Batch b[2];
+  uint32_t s = wave;
+  load(b[0], s);
+  for (; s < slabs; s += 2 * U * NW) {
+    load(b[1], s + U * NW);
+    multiply(b[0], s);
+    load(b[0], s + 2 * U * NW);
+    multiply(b[1], s + U * NW);
+  }
+#pragma unroll
+  for (int r = 0; r < RN; r++)
+#pragma unroll
+    for (int f = 0; f < FM; f++)
+      if (f == 0 || (uint32_t)f < live) lds[wave][r * FM + f][lane] = acc[r][f];
+  __syncthreads();
+  for (uint32_t q = wave; q < RN * FM; q += NW) {
+    const uint32_t r = q / FM, f = q % FM;
+    if (f >= live) continue;
+    f32x4 sum = lds[0][q][lane];
+#pragma unroll
+    for (int w = 1; w < NW; w++) sum += lds[w][q][lane];
+    const uint32_t m = t.m0 + 16 * f + i;
+    if (m < t.mEnd) {
+      const float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+      storeRun((Out *)a.y + (size_t)m * a.ldy, t.n0 + 16 * r + 4 * g, a.n, v);
+    }
+  }
+}
+
 // ------------------------------------------------------------- launch tables
 
 enum ProductForm { kFormNK = 0, kFormKN = 1, kFormDw = 2 };
@@ -683,20 +817,28 @@ flagcxResult_t launchProductBf16(const ProductArgs &a, int form, bool outF32, hi
 flagcxResult_t launchProductF16(const ProductArgs &a, int form, bool outF32, hipStream_t s);
 flagcxResult_t launchProductE4m3(const ProductArgs &a, int outDtype, hipStream_t s);
 
-template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW, bool DIRECT>
-flagcxResult_t launchTiles(ProductArgs a, hipStream_t s) {
-  a.nTiles = (a.n + BN - 1) / BN;
-  if (DW) a.mTiles = (a.m + BM - 1) / BM;
-  else if (!a.offsets) a.mTiles = (a.rows + BM - 1) / BM;
-  else a.mTiles = a.rows / BM + (a.experts < a.rows ? a.experts : a.rows);   // every expert's last tile may be partial
-  const uint64_t grid = (uint64_t)a.nTiles * a.mTiles * (DW ? a.experts : 1);
+inline flagcxResult_t launchGrid(const void *kernel, ProductArgs &a, uint32_t bn, uint32_t bm, bool dw, uint32_t threads, hipStream_t s) {
+  a.nTiles = (a.n + bn - 1) / bn;
+  if (dw) a.mTiles = (a.m + bm - 1) / bm;
+  else if (!a.offsets) a.mTiles = (a.rows + bm - 1) / bm;
+  else a.mTiles = a.rows / bm + (a.experts < a.rows ? a.experts : a.rows);   // every expert's last tile may be partial
+  const uint64_t grid = (uint64_t)a.nTiles * a.mTiles * (dw ? a.experts : 1);
   if (grid > 0x7fffffffu) return flagcxNotSupported;
   void *argv[] = {&a};
+  return hipLaunchKernel(kernel, dim3((uint32_t)grid), dim3(threads), argv, 0, s) == hipSuccess ? flagcxSuccess : flagcxUnhandledDeviceError;
+}
+
+template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW, bool DIRECT>
+flagcxResult_t launchTiles(ProductArgs a, hipStream_t s) {
   const void *kernel;
   if constexpr (DIRECT) kernel = reinterpret_cast<const void *>(productDirect<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
   else kernel = reinterpret_cast<const void *>(productGuarded<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
-  return hipLaunchKernel(kernel, dim3((uint32_t)grid), dim3(WN * WM * 64), argv, 0, s) == hipSuccess ? flagcxSuccess
-                                                                                                   : flagcxUnhandledDeviceError;
+  return launchGrid(kernel, a, BN, BM, DW, WN * WM * 64, s);
+}
+
+template <class T, class Out, int RN, int FM, int NW, int U>
+flagcxResult_t launchThin(ProductArgs a, hipStream_t s) {
+  return launchGrid(reinterpret_cast<const void *>(productThin<T, Out, RN, FM, NW, U>), a, 16 * RN, 16 * FM, false, NW * 64, s);
 }
 
 // Whole 16-byte chunks everywhere: what the direct kernels assume.  `inner` is the
@@ -709,6 +851,11 @@ inline bool wholeChunks(const void *p, size_t ld, size_t expert, size_t inner, s
 template <class T, class Out, bool NACROSS, bool MACROSS, bool DW>
 flagcxResult_t launchShapes(const ProductArgs &a, hipStream_t s) {
   const size_t es = kBytes<T>;
+  if constexpr (!NACROSS && !DW) {
+    const uint64_t each = a.rows / (a.experts ? a.experts : 1);
+    if (each <= 4) return launchThin<T, Out, 2, 1, 8, kBytes<T> == 1 ? 2 : 4>(a, s);
+    if (each <= 48) return launchThin<T, Out, 2, 4, 8, 1>(a, s);
+  }
   const bool direct = wholeChunks(a.pn, a.ldn, a.expertN, NACROSS ? a.n : a.k, es) &&
                       wholeChunks(a.pm, a.ldm, 0, MACROSS ? a.m : a.k, es);
   if (!direct) return launchTiles<T, Out, 128, 128, 2, 2, NACROSS, MACROSS, DW, false>(a, s);
