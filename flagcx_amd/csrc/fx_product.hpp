@@ -74,20 +74,19 @@ __device__ __forceinline__ uint32_t waveScan(uint32_t v) {   // inclusive prefix
   return v;
 }
 
-// Tiles of BM rows that expert e's rows make.
-template <int BM>
-__device__ __forceinline__ uint32_t tilesOf(const ProductArgs &a, uint32_t e, uint32_t *first, uint32_t *last) {
-  *first = *last = 0;
+// Rows of expert e.
+__device__ __forceinline__ uint32_t rowsOf(const ProductArgs &a, uint32_t e, uint32_t *first) {
+  *first = 0;
   if (e >= a.experts) return 0;
   *first = bound(a, e);
-  *last = bound(a, e + 1);
-  return *last > *first ? (*last - *first + BM - 1) / BM : 0;
+  const uint32_t last = bound(a, e + 1);
+  return last > *first ? last - *first : 0;
 }
 
 // Consecutive tiles of one die (workgroups go to the eight dies in turn) are made
 // neighbours: a die's L2 then holds the operands of a block of kPanel row tiles by
 // a few column tiles.
-constexpr uint32_t kDies = 8, kPanel = 8;
+constexpr uint32_t kDies = 8, kPanel = 8, kGroup = 4, kUnits = 256;
 __device__ __forceinline__ uint32_t dieOrder(uint32_t id, uint32_t total) {
   const uint32_t die = id % kDies, at = id / kDies, q = total / kDies, r = total % kDies;
   return die * q + (die < r ? die : r) + at;
@@ -101,54 +100,87 @@ __device__ __forceinline__ void panelOrder(uint32_t id, uint32_t mTiles, uint32_
 
 // The row tiles of all experts are counted on the device (the host knows only an
 // upper bound, the grid): every wavefront scans the boundaries, 64 experts at a time.
-template <int BN, int BM>
+// ORDERED: kGroup columns of tiles at a time, first the whole tiles of all experts,
+// then the experts' last tiles with more than half their rows, then the others, which
+// take half the time and fill up the end of the call.  A group's weights are used by
+// both while the memory-side cache holds them.
+template <int BN, int BM, bool ORDERED>
 __device__ __forceinline__ bool findTile(const ProductArgs &a, Tile *t) {
-  uint32_t mTiles, mt, nt;
+  uint32_t mt, nt, id = blockIdx.x;
   if (!a.offsets) {
-    mTiles = (a.rows + BM - 1) / BM;
-    if (blockIdx.x >= mTiles * a.nTiles) return false;
-    panelOrder(dieOrder(blockIdx.x, mTiles * a.nTiles), mTiles, a.nTiles, &mt, &nt);
+    const uint32_t mTiles = (a.rows + BM - 1) / BM;
+    if (id >= mTiles * a.nTiles) return false;
+    panelOrder(dieOrder(id, mTiles * a.nTiles), mTiles, a.nTiles, &mt, &nt);
     *t = Tile{0, mt * BM, a.rows, nt * BN, 0, a.k};
     return true;
   }
   const uint32_t lane = threadIdx.x & 63;
-  uint32_t first, last, scan = 0;
-  mTiles = 0;
+  uint32_t first = 0, rows = 0, scan = 0, tiles[3] = {0, 0, 0};
+  // Tiles of kind 0 of this lane's expert; kinds 1 and 2 are one at most.
+  auto whole = [&] { return ORDERED ? rows / BM : (rows + BM - 1) / BM; };
+  auto isKind = [&](int k) { return ORDERED && rows % BM != 0 && (rows % BM > BM / 2) == (k == 1); };
   for (uint32_t e = 0; e < a.experts; e += 64) {
-    scan = waveScan(tilesOf<BM>(a, e + lane, &first, &last));
-    mTiles += uniform((uint32_t)__shfl((int)scan, 63));
+    rows = rowsOf(a, e + lane, &first);
+    scan = waveScan(whole());
+    tiles[0] += uniform((uint32_t)__shfl((int)scan, 63));
+    tiles[1] += (uint32_t)__popcll(__ballot(isKind(1)));
+    tiles[2] += (uint32_t)__popcll(__ballot(isKind(2)));
   }
-  if (mTiles > a.mTiles) mTiles = a.mTiles;          // boundaries that are not ascending: the grid ends here
-  if (blockIdx.x >= mTiles * a.nTiles) return false;
-  panelOrder(dieOrder(blockIdx.x, mTiles * a.nTiles), mTiles, a.nTiles, &mt, &nt);
-  uint32_t before = 0;
-  for (uint32_t e = 0; e < a.experts; e += 64) {
-    if (a.experts > 64) scan = waveScan(tilesOf<BM>(a, e + lane, &first, &last));
-    const uint32_t all = uniform((uint32_t)__shfl((int)scan, 63));
-    if (mt < before + all) {
-      const uint64_t over = __ballot(before + scan > mt);
-      const uint32_t l = (uint32_t)__builtin_ctzll(over);
-      const uint32_t prev = l ? uniform((uint32_t)__shfl((int)scan, (int)(l - 1))) : 0;
-      const uint32_t f = uniform((uint32_t)__shfl((int)first, (int)l));
-      *t = Tile{e + l, f + (mt - before - prev) * BM, uniform((uint32_t)__shfl((int)last, (int)l)), nt * BN, 0, a.k};
+  const uint32_t mTiles = tiles[0] + tiles[1] + tiles[2];
+  if (id >= mTiles * a.nTiles) return false;
+  const uint32_t wide = ORDERED ? kGroup : a.nTiles, group = id / (mTiles * wide);
+  const uint32_t left = a.nTiles - group * wide, w = left < wide ? left : wide;   // columns of tiles in this group
+  id -= group * mTiles * wide;
+  int kind = 0;
+  while (kind < 2 && id >= tiles[kind] * w) id -= tiles[kind++] * w;
+  const uint32_t at = dieOrder(id, tiles[kind] * w);
+  mt = at / w;
+  nt = group * wide + at % w;
+  for (uint32_t e = 0, before = 0; e < a.experts; e += 64) {
+    if (a.experts > 64) {
+      rows = rowsOf(a, e + lane, &first);
+      scan = waveScan(whole());
+    }
+    const uint64_t set = __ballot(isKind(kind));
+    const uint32_t here = kind ? (uint32_t)__popcll(set) : uniform((uint32_t)__shfl((int)scan, 63));
+    if (mt < before + here) {
+      const uint32_t want = mt - before;             // which of this kind's tiles among the 64 experts
+      const uint32_t ahead = kind ? (uint32_t)__builtin_amdgcn_mbcnt_hi((uint32_t)(set >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0))
+                                  : scan - whole();
+      const bool mine = kind ? isKind(kind) && ahead == want : ahead <= want && want < scan;
+      const uint32_t l = (uint32_t)__builtin_ctzll(__ballot(mine));
+      const uint32_t skip = kind ? rows / BM : want - ahead;                // tiles of the same expert in front
+      const uint32_t f = uniform((uint32_t)__shfl((int)first, (int)l)), r = uniform((uint32_t)__shfl((int)rows, (int)l));
+      *t = Tile{e + l, f + uniform((uint32_t)__shfl((int)skip, (int)l)) * BM, f + r, nt * BN, 0, a.k};
       return true;
     }
-    before += all;
+    before += here;
   }
   return false;
 }
 
+// Experts differ in length, so each one's tiles are dealt to all dies, and the
+// longest expert's come first (up to 64 experts; more are taken as they lie).
 template <int BN, int BM>
 __device__ __forceinline__ bool findTileDw(const ProductArgs &a, Tile *t) {
-  // Experts differ in length, so each one's tiles are dealt to all dies.
-  const uint32_t per = a.mTiles * a.nTiles, e = blockIdx.x / per;
-  uint32_t mt, nt, first = 0, last = a.rows;
-  panelOrder(dieOrder(blockIdx.x - e * per, per), a.mTiles, a.nTiles, &mt, &nt);
+  const uint32_t per = a.mTiles * a.nTiles, turn = blockIdx.x / per;
+  uint32_t mt, nt, e = turn, first = 0, rows = a.rows;
+  panelOrder(dieOrder(blockIdx.x - turn * per, per), a.mTiles, a.nTiles, &mt, &nt);
   if (a.offsets) {
-    first = uniform(bound(a, e));
-    last = uniform(bound(a, e + 1));
+    if (a.experts <= 64) {
+      const uint32_t lane = threadIdx.x & 63;
+      rows = rowsOf(a, lane, &first);
+      uint32_t rank = 0;
+      for (uint32_t j = 0; j < a.experts; j++) {
+        const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)rows, (int)j);
+        rank += other > rows || (other == rows && j < lane);
+      }
+      e = (uint32_t)__builtin_ctzll(__ballot(lane < a.experts && rank == turn));
+    }
+    rows = uniform(rowsOf(a, e, &first));
+    first = uniform(first);
   }
-  *t = Tile{e, mt * BM, a.m, nt * BN, first, last > first ? last - first : 0};
+  *t = Tile{e, mt * BM, a.m, nt * BN, first, rows};
   return true;
 }
 
@@ -172,6 +204,12 @@ struct Side {
   static constexpr int kElems = 16 / ES;
   static constexpr uint32_t kSlab = 128 / ES;            // reduction elements per slab
 
+  // A thread's chunks lie in rows that the exchange treats alike, except where its
+  // rows are 16 apart on the n side.
+  static constexpr bool kTurns = NSIDE && !ACROSS && kStep % 32 != 0;
+  static_assert(ACROSS ? kStep % 4 == 0 : kStep % 16 == 0, "rows that the exchange treats alike");
+  __device__ __forceinline__ uint32_t element(int q) const { return (chunk ^ (kTurns && (q & 1) ? 4u : 0u)) * kElems; }
+
   // position of this thread's first chunk
   uint32_t row, chunk;
   __device__ __forceinline__ void init() {
@@ -184,7 +222,7 @@ struct Side {
   // index 0 at reduction 0.  own / red: how much of the tile's own index and of the
   // slab's reduction exists.
   __device__ __forceinline__ u32x4 guarded(const char *base, size_t ld, int i, uint32_t own, uint32_t red) const {
-    const uint32_t r = row + i * kStep, c = chunk * kElems;
+    const uint32_t r = row + i * kStep, c = element(i);
     u32x4 v = {};
     const uint32_t rows = ACROSS ? red : own, cols = ACROSS ? own : red;
     if (r >= rows || c >= cols) return v;
@@ -409,7 +447,7 @@ __global__ void __launch_bounds__(WN *WM * 64) productGuarded(ProductArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[P::kLdsN + P::kLdsM];
   char *ln = lds, *lm = lds + P::kLdsN;
   Tile t;
-  if (!(DW ? findTileDw<BN, BM>(a, &t) : findTile<BN, BM>(a, &t))) return;
+  if (!(DW ? findTileDw<BN, BM>(a, &t) : findTile<BN, BM, true>(a, &t))) return;
   P p;
   p.init();
   typename P::N sn;
@@ -462,8 +500,11 @@ constexpr uint32_t kOutside = 0x80000000u;
 __device__ __forceinline__ void loadToLds(uint32_t ldsAt, uint32_t voff, __amdgpu_buffer_rsrc_t rsrc, uint32_t soff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(ldsAt), "v"(voff), "s"(rsrc), "s"(soff));
 }
+// `left` = loads of this wavefront that may still be on their way.
+template <int left>
 __device__ __forceinline__ void waitAndMeet() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  static_assert(left < 64, "six bits of counter");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(left) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -479,17 +520,16 @@ struct DirectSide : Side<R, NT, ES, ACROSS, NSIDE> {
     step = uniform((uint32_t)(S::kStep * ld * ES));
     at = (uint64_t)(uintptr_t)base;
     advance = ACROSS ? S::kSlab * ld * ES : 128;
-    const uint32_t off = (uint32_t)((S::row * ld + S::chunk * S::kElems) * ES);
 #pragma unroll
     for (int q = 0; q < S::kLoads; q++)
-      voff[q] = (ACROSS ? S::chunk * S::kElems < own : S::row + q * S::kStep < own) ? off : kOutside;
+      voff[q] = (ACROSS ? S::element(q) < own : S::row + q * S::kStep < own) ? (uint32_t)((S::row * ld + S::element(q)) * ES) : kOutside;
   }
   // red: reduction elements left from this slab on
   __device__ __forceinline__ void issue(uint32_t lds, uint32_t wave, uint32_t red) {
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)at, 0, 0x7fffffff, 0x00020000);
 #pragma unroll
     for (int q = 0; q < S::kLoads; q++) {
-      const bool there = ACROSS ? S::row + q * S::kStep < red : S::chunk * S::kElems < red;
+      const bool there = ACROSS ? S::row + q * S::kStep < red : S::element(q) < red;
       loadToLds(lds + (q * NT + wave * 64) * 16, there ? voff[q] : kOutside, rsrc, q * step);
     }
     at += advance;
@@ -497,7 +537,8 @@ struct DirectSide : Side<R, NT, ES, ACROSS, NSIDE> {
 };
 
 // The e4m3 rows' scales of one slab, one float per row of the tile, brought to LDS
-// in the order in which a lane wants them (its fragments' rows side by side).
+// in the order in which a lane wants them (its fragments' rows side by side).  Every
+// wavefront issues one load, also those without a row, so that all count alike.
 template <int BM, int TM>
 struct DirectScales {
   static constexpr uint32_t FM = TM / 16;
@@ -509,11 +550,9 @@ struct DirectScales {
     at = (uint64_t)(uintptr_t)base;
   }
   __device__ __forceinline__ void issue(uint32_t lds, uint32_t wave, bool there) {
-    if (wave * 64 < BM) {
-      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)at, 0, 0x7fffffff, 0x00020000);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds + wave * 256),
-                   "v"(there ? voff : kOutside), "s"(rsrc));
-    }
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)at, 0, 0x7fffffff, 0x00020000);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds + wave * 256),
+                 "v"(there ? voff : kOutside), "s"(rsrc));
     at += 4;
   }
 };
@@ -521,9 +560,10 @@ struct DirectScales {
 // The slabs as a pipeline.  A slab is multiplied in phases; the fragments of
 // the next phase are read from LDS while this one's are multiplied.  In front of
 // the last phase all of a slab's fragments are in registers: there the wavefronts
-// meet, its buffer is handed to the loads of the slab after the next, and the next
-// slab, whose loads have had a whole slab's time, is read from.  Loads past the
-// last slab have no lanes inside the buffer and read nothing.
+// meet, its buffers are handed to the loads of slabs further on, and the next
+// slab, whose loads have had SN - 1 and SM - 1 slabs' time, is read from.  (Weights
+// come from memory more often than rows do, and have the deeper ring where LDS
+// allows.)  Loads past the last slab have no lanes inside the buffer and read nothing.
 //
 // 16 bits: two halves of the reduction, each with two groups of m fragments.
 // e4m3: a phase is one m fragment (registers: 128 of accumulators, 32 of n
@@ -531,16 +571,17 @@ struct DirectScales {
 // accumulators two products later, in the shadow of the matrix instructions.
 #define FX_FENCE() __builtin_amdgcn_sched_barrier(0)
 
-template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW>
+template <class T, class Out, int BN, int BM, int WN, int WM, int SN, int SM, bool NACROSS, bool MACROSS, bool DW>
 __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
   using P = Product<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>;
-  constexpr uint32_t kScales = P::kScaled ? 1024 : 0, kStage = P::kLdsN + P::kLdsM + kScales;
-  static_assert(BM <= 256, "room for the scales");
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+  constexpr uint32_t kStageM = P::kLdsM + (P::kScaled ? P::kThreads * 4 : 0), kLds = SN * P::kLdsN + SM * kStageM;
+  constexpr int kLoadsN = P::N::kLoads, kLoadsM = P::M::kLoads + P::kScaled;   // per thread and slab
+  static_assert(BM <= P::kThreads && SN >= SM && SM >= 2, "a thread per row's scale");
+  __shared__ __attribute__((aligned(1024))) char lds[kLds];
   typedef __attribute__((address_space(3))) char *ldsPtr;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(ldsPtr)lds;
   Tile t;
-  if (!(DW ? findTileDw<BN, BM>(a, &t) : findTile<BN, BM>(a, &t))) return;
+  if (!(DW ? findTileDw<BN, BM>(a, &t) : findTile<BN, BM, true>(a, &t))) return;
   P p;
   p.init();
   const uint32_t wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -558,25 +599,43 @@ __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
     blockScale = a.sn + (size_t)t.expert * a.expertSn + (size_t)(b < last ? b : last) * a.ldsn;
   }
   const uint32_t slabs = (t.kLen + P::kSlab - 1) / P::kSlab;
-  uint32_t red = t.kLen;
-  auto issue = [&](uint32_t s) {
-    const uint32_t at = lds0 + (s & 1) * kStage;
-    sn.issue(at, wave, red);
-    sm.issue(at + P::kLdsN, wave, red);
-    if constexpr (P::kScaled) ss.issue(at + P::kLdsN + P::kLdsM, wave, red != 0);
-    red = red > P::kSlab ? red - P::kSlab : 0;
+  // The slabs s + SM of the m side and s + SN of the n side, into the buffers of slab s.
+  uint32_t curN = 0, curM = SN * P::kLdsN, leftN = t.kLen, leftM = t.kLen;
+  auto issueN = [&] {
+    sn.issue(lds0 + curN, wave, leftN);
+    leftN = leftN > P::kSlab ? leftN - P::kSlab : 0;
+    curN = curN + P::kLdsN < SN * P::kLdsN ? curN + P::kLdsN : 0;
+  };
+  auto issueM = [&] {
+    sm.issue(lds0 + curM, wave, leftM);
+    if constexpr (P::kScaled) ss.issue(lds0 + curM + P::kLdsM, wave, leftM != 0);
+    leftM = leftM > P::kSlab ? leftM - P::kSlab : 0;
+    curM = curM + kStageM < kLds ? curM + kStageM : SN * P::kLdsN;
   };
   if (slabs) {
-    issue(0);
-    waitAndMeet();
-    issue(1);
+#pragma unroll
+    for (int q = 0; q < SN; q++) {
+      if (q < SM) issueM();
+      issueN();
+    }
+    waitAndMeet<(SM - 1) * kLoadsM + (SN - 1) * kLoadsN>();
+    const char *ln = lds, *lm = lds + SN * P::kLdsN;
+    auto nextSlab = [&] {
+      FX_FENCE();
+      waitAndMeet<(SM - 2) * kLoadsM + (SN - 2) * kLoadsN>();
+      issueM();
+      issueN();
+      ln = lds + curN;
+      lm = lds + curM;
+    };
+    if (t.m0 + p.wm >= t.mEnd) {              // an expert's last tile: no row for this wavefront
+      for (uint32_t s = 0; s < slabs; s++) nextSlab();
+    } else
     if constexpr (P::kScaled) {
       u32x4 n[P::FN][2], m[2][2];
       f32x4 part[3];
       float scale[2];
-      uint32_t cur = 0;
       float blocks = 0.f;                     // lane l: the block's scale of slab 64 * (s / 64) + l
-      const char *ln = lds, *lm = lds + P::kLdsN;
       auto readM = [&](int q) {
         const int fragment = q % P::FM;
         m[q & 1][0] = p.readM(lm, fragment, 0);
@@ -602,14 +661,7 @@ __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
         };
 #pragma unroll
         for (int q = 0; q < P::FM; q++) {
-          if (q == P::FM - 1) {
-            FX_FENCE();
-            waitAndMeet();
-            issue(s + 2);
-            cur ^= kStage;                    // kStage or 0
-            ln = lds + cur;
-            lm = ln + P::kLdsN;
-          }
+          if (q == P::FM - 1) nextSlab();
           FX_FENCE();
           w[q] = scale[q & 1] * sb;
           readM(q + 1);                       // FM is even: FM is fragment 0 of the next slab, in buffer 0
@@ -629,8 +681,6 @@ __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
     } else {
       constexpr int GQ = P::FM / 2;
       u32x4 n[2][P::FN], m[2][GQ];
-      uint32_t cur = 0;
-      const char *ln = lds, *lm = lds + P::kLdsN;
       auto readN = [&](int half) {
 #pragma unroll
         for (int f = 0; f < P::FN; f++) n[half][f] = p.readN(ln, f, half);
@@ -644,14 +694,7 @@ __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
       for (uint32_t s = 0; s < slabs; s++) {
 #pragma unroll
         for (int ph = 0; ph < 4; ph++) {
-          if (ph == 3) {
-            FX_FENCE();
-            waitAndMeet();
-            issue(s + 2);
-            cur ^= kStage;
-            ln = lds + cur;
-            lm = ln + P::kLdsN;
-          }
+          if (ph == 3) nextSlab();
           FX_FENCE();
           readM((ph + 1) & 3);
           if (ph == 0) readN(1);
@@ -678,121 +721,185 @@ __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
 // memory bounds the call.  A workgroup owns 16 RN columns of the output and up to
 // 16 FM rows; its wavefronts share the reduction, slab by slab in turn (so that
 // together they read long runs of each weight row), and their partial sums meet
-// in LDS in a fixed order.  Fragments without a row are skipped.  U slabs are
-// loaded while U are multiplied.  e4m3 operands are widened to bf16, whose sums are
-// those of fp32: the matrix cores have time.
-template <class T, class Out, int RN, int FM, int NW, int U>
-__global__ void __launch_bounds__(NW * 64) productThin(ProductArgs a) {
-  constexpr int BN = 16 * RN, BM = 16 * FM, ES = kBytes<T>, kElems = 16 / ES;
-  constexpr bool kScaled = ES == 1;
-  constexpr uint32_t kSlab = 128 / ES;
-  __shared__ f32x4 lds[NW][RN * FM][64];
-  Tile t;
-  if (!findTile<BN, BM>(a, &t)) return;
-  const uint32_t wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  const uint32_t own = t.mEnd - t.m0, live = own >= (uint32_t)BM ? FM : (own + 15) / 16;
-  const uint32_t slabs = (a.k + kSlab - 1) / kSlab;
-  const char *pw[RN], *px[FM];
-  bool xHere[FM];
-#pragma unroll
-  for (int r = 0; r < RN; r++) {
-    const uint32_t n = t.n0 + 16 * r + i;      // columns behind the last repeat it; they are not stored
-    pw[r] = (const char *)a.pn + ((size_t)t.expert * a.expertN + (size_t)(n < a.n ? n : a.n - 1) * a.ldn) * ES;
-  }
-#pragma unroll
-  for (int f = 0; f < FM; f++) {
-    xHere[f] = 16 * f + i < own;
-    px[f] = (const char *)a.pm + (size_t)(t.m0 + 16 * f + (xHere[f] ? i : 0)) * a.ldm * ES;
-  }
-  const float *ps = nullptr, *pb = nullptr;
-  if constexpr (kScaled) {
-    ps = a.sm + (size_t)t.m0 * a.ldsm;
-    pb = a.sn + (size_t)t.expert * a.expertSn;
-  }
-  f32x4 acc[RN][FM];
-#pragma unroll
-  for (int r = 0; r < RN; r++)
-#pragma unroll
-    for (int f = 0; f < FM; f++) acc[r][f] = f32x4{};
+// in LDS in a fixed order.  U slabs are loaded while U are multiplied, without a
+// branch: lanes without a row, a column or a slab load from outside the buffer,
+// which touches no memory and gives zeros.  Each tile starts at another slab,
+// because tiles that walk rows a power of two apart in step meet on the same
+// memory channels (one token through 8 of 64 experts 28.9 -> 26.1 us).  e4m3
+// operands are widened to bf16, whose sums are those of fp32: the matrix cores
+// have time.
+__device__ __forceinline__ u32x4 loadRaw16(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, (int)soff, 0));
+}
+__device__ __forceinline__ float loadRaw4(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)voff, (int)soff, 0));
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t bufferAt(const void *p) {
+  const uint64_t at = (uint64_t)(uintptr_t)p;
+  const uint64_t u = (uint64_t)uniform((uint32_t)at) | ((uint64_t)uniform((uint32_t)(at >> 32)) << 32);
+  return __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)u, 0, 0x7fffffff, 0x00020000);
+}
 
+template <class T, int RN, int FM, int NW, int U>
+struct Thin {
+  static constexpr int ES = kBytes<T>, kElems = 16 / ES;
+  static constexpr bool kScaled = ES == 1;
+  static constexpr uint32_t kSlab = 128 / ES;
   struct Batch {
     u32x4 w[U][RN][2], x[U][FM][2];
     float sx[U][FM], sb[U][RN];
   };
-  auto chunk = [&](const char *p, uint32_t c, bool tail) -> u32x4 {
-    if (!tail || (c + 1) * kElems <= a.k) return *reinterpret_cast<const u32x4_anywhere *>(p + c * 16);
-    u32x4 v = {};
-#pragma unroll
-    for (int j = 0; j < kElems; j++)
-      if (c * kElems + j < a.k) {
-        if constexpr (ES == 2) v[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(p)[c * kElems + j] << (16 * (j & 1));
-        else v[j >> 2] |= (uint32_t)reinterpret_cast<const uint8_t *>(p)[c * kElems + j] << (8 * (j & 3));
-      }
-    return v;
-  };
-  // slabs s, s + NW, ...; the reduction's last slab may be partial
-  auto load = [&](Batch &b, uint32_t s0) {
+  f32x4 acc[RN][FM];
+  __amdgpu_buffer_rsrc_t bw, bx, bs, bb;
+  uint32_t ow[RN], ox[FM], os[FM], ob[RN];
+  uint32_t full, turn;            // whole slabs; the slab this tile starts at
+
+  __device__ __forceinline__ void load(Batch &b, uint32_t s0) const {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const uint32_t s = s0 + u * NW;
-      if (s >= slabs) continue;
-      const bool tail = (s + 1) * kSlab > a.k;
+      uint32_t s = s0 + u * NW;
+      const uint32_t out = s < full ? 0 : kOutside;
+      s += turn;
+      s = s >= full ? s - full : s;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const uint32_t c = s * 8 + h * 4 + g;
 #pragma unroll
-        for (int r = 0; r < RN; r++) b.w[u][r][h] = chunk(pw[r], c, tail);
+        for (int r = 0; r < RN; r++) b.w[u][r][h] = loadRaw16(bw, (ow[r] + h * 64) | out, s * 128);
 #pragma unroll
-        for (int f = 0; f < FM; f++)
-          if (f == 0 || (uint32_t)f < live) {
-            b.x[u][f][h] = u32x4{};
-            if (xHere[f]) b.x[u][f][h] = chunk(px[f], c, tail);
-          }
+        for (int f = 0; f < FM; f++) b.x[u][f][h] = loadRaw16(bx, (ox[f] + h * 64) | out, s * 128);
       }
       if constexpr (kScaled) {
 #pragma unroll
-        for (int f = 0; f < FM; f++)
-          if (f == 0 || (uint32_t)f < live) b.sx[u][f] = xHere[f] ? ps[(size_t)(16 * f + i) * a.ldsm + s] : 0.f;
+        for (int f = 0; f < FM; f++) b.sx[u][f] = loadRaw4(bs, os[f] | out, s * 4);
 #pragma unroll
-        for (int r = 0; r < RN; r++) b.sb[u][r] = pb[(size_t)((t.n0 + 16 * r < a.n ? t.n0 + 16 * r : a.n - 1) / FX_SCALE_GROUP) * a.ldsn + s];
+        for (int r = 0; r < RN; r++) b.sb[u][r] = loadRaw4(bb, ob[r] | out, s * 4);
       }
     }
-  };
-  auto multiply = [&](const Batch &b, uint32_t s0) {
+  }
+  __device__ __forceinline__ void multiply(const Batch &b) {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      if (s0 + u * NW >= slabs) continue;
+    for (int u = 0; u < U; u++)
 #pragma unroll
       for (int f = 0; f < FM; f++)
-        if (f == 0 || (uint32_t)f < live)
 #pragma unroll
-          for (int r = 0; r < RN; r++) {
-            if constexpr (kScaled) {
-              const f32x4 p = mma8<E4m3Exact>(b.w[u][r], b.x[u][f]);
-              const float sc = b.sx[u][f] * b.sb[u][r];
+        for (int r = 0; r < RN; r++) {
+          if constexpr (kScaled) {
+            const f32x4 p = mma8<E4m3Exact>(b.w[u][r], b.x[u][f]);
+            const float sc = b.sx[u][f] * b.sb[u][r];
 #pragma unroll
-              for (int v = 0; v < 4; v++) acc[r][f][v] = __builtin_fmaf(p[v], sc, acc[r][f][v]);
-            } else {
+            for (int v = 0; v < 4; v++) acc[r][f][v] = __builtin_fmaf(p[v], sc, acc[r][f][v]);
+          } else {
 #pragma unroll
-              for (int h = 0; h < 2; h++) acc[r][f] = mma<T>(b.w[u][r][h], b.x[u][f][h], acc[r][f]);
-            }
+            for (int h = 0; h < 2; h++) acc[r][f] = mma<T>(b.w[u][r][h], b.x[u][f][h], acc[r][f]);
           }
-    }
-  };
-  Batch b[2];
-  uint32_t s = wave;
-  load(b[0], s);
-  for (; s < slabs; s += 2 * U * NW) {
-    load(b[1], s + U * NW);
-    multiply(b[0], s);
-    load(b[0], s + 2 * U * NW);
-    multiply(b[1], s + U * NW);
+        }
   }
+  // 16 bytes of a row from element c on, of which `cols` exist
+  __device__ __forceinline__ static u32x4 part(const char *row, uint32_t c, uint32_t cols) {
+    u32x4 v = {};
 #pragma unroll
-  for (int r = 0; r < RN; r++)
+    for (int j = 0; j < kElems; j++)
+      if (c + j < cols) {
+        if constexpr (ES == 2) v[j >> 1] |= (uint32_t) reinterpret_cast<const uint16_t *>(row)[c + j] << (16 * (j & 1));
+        else v[j >> 2] |= (uint32_t) reinterpret_cast<const uint8_t *>(row)[c + j] << (8 * (j & 3));
+      }
+    return v;
+  }
+
+  __device__ __forceinline__ void run(const ProductArgs &a, const Tile &t, uint32_t wave, uint32_t i, uint32_t g) {
+    const uint32_t own = t.mEnd - t.m0;
+    full = a.k / kSlab;
+    turn = full ? (t.n0 / (16 * RN) * 37 + t.expert * 11) % full : 0;
+    const char *w0 = (const char *)a.pn + ((size_t)t.expert * a.expertN + (size_t)t.n0 * a.ldn) * ES;
+    const char *x0 = (const char *)a.pm + (size_t)t.m0 * a.ldm * ES;
+    bw = bufferAt(w0);
+    bx = bufferAt(x0);
 #pragma unroll
-    for (int f = 0; f < FM; f++)
-      if (f == 0 || (uint32_t)f < live) lds[wave][r * FM + f][lane] = acc[r][f];
+    for (int r = 0; r < RN; r++)
+      ow[r] = t.n0 + 16 * r + i < a.n ? (uint32_t)((16 * r + i) * a.ldn * ES) + g * 16 : kOutside;
+#pragma unroll
+    for (int f = 0; f < FM; f++) ox[f] = 16 * f + i < own ? (uint32_t)((16 * f + i) * a.ldm * ES) + g * 16 : kOutside;
+    const float *s0 = nullptr, *b0 = nullptr;
+    if constexpr (kScaled) {
+      s0 = a.sm + (size_t)t.m0 * a.ldsm;
+      b0 = a.sn + (size_t)t.expert * a.expertSn;
+      bs = bufferAt(s0);
+      bb = bufferAt(b0);
+#pragma unroll
+      for (int f = 0; f < FM; f++) os[f] = 16 * f + i < own ? (uint32_t)((16 * f + i) * a.ldsm * 4) : kOutside;
+#pragma unroll
+      for (int r = 0; r < RN; r++) ob[r] = t.n0 + 16 * r < a.n ? (uint32_t)((t.n0 + 16 * r) / FX_SCALE_GROUP * a.ldsn * 4) : kOutside;
+    }
+#pragma unroll
+    for (int r = 0; r < RN; r++)
+#pragma unroll
+      for (int f = 0; f < FM; f++) acc[r][f] = f32x4{};
+    Batch b[2];
+    load(b[0], wave);
+    for (uint32_t s = wave; s < full; s += 2 * U * NW) {
+      load(b[1], s + U * NW);
+      multiply(b[0]);
+      load(b[0], s + 2 * U * NW);
+      multiply(b[1]);
+    }
+    // what is left behind the whole slabs: one wavefront, element by element
+    if (a.k % kSlab && wave == full % NW) {
+      Thin<T, RN, FM, NW, 1> last;
+      typename Thin<T, RN, FM, NW, 1>::Batch e;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint32_t c = full * kSlab + (h * 4 + g) * kElems;
+#pragma unroll
+        for (int r = 0; r < RN; r++)
+          e.w[0][r][h] = ow[r] < kOutside ? part(w0 + (size_t)(16 * r + i) * a.ldn * ES, c, a.k) : u32x4{};
+#pragma unroll
+        for (int f = 0; f < FM; f++)
+          e.x[0][f][h] = ox[f] < kOutside ? part(x0 + (size_t)(16 * f + i) * a.ldm * ES, c, a.k) : u32x4{};
+      }
+      if constexpr (kScaled) {
+#pragma unroll
+        for (int f = 0; f < FM; f++) e.sx[0][f] = loadRaw4(bs, os[f], full * 4);
+#pragma unroll
+        for (int r = 0; r < RN; r++) e.sb[0][r] = loadRaw4(bb, ob[r], full * 4);
+      }
+#pragma unroll
+      for (int r = 0; r < RN; r++)
+#pragma unroll
+        for (int f = 0; f < FM; f++) last.acc[r][f] = acc[r][f];
+      last.multiply(e);
+#pragma unroll
+      for (int r = 0; r < RN; r++)
+#pragma unroll
+        for (int f = 0; f < FM; f++) acc[r][f] = last.acc[r][f];
+    }
+  }
+};
+
+// FM = 4 holds three bodies, for 16, 32 and 64 rows: what of a tile exists is
+// known on the device only.
+template <class T, class Out, int RN, int FM, int NW, int U>
+__global__ void __launch_bounds__(NW * 64) productThin(ProductArgs a) {
+  __shared__ f32x4 lds[NW][RN * FM][64];
+  Tile t;
+  if (!findTile<16 * RN, 16 * FM, false>(a, &t)) return;
+  const uint32_t wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const uint32_t own = t.mEnd - t.m0, live = own >= 16 * FM ? FM : (own + 15) / 16;
+  auto body = [&](auto rows) {
+    constexpr int F = decltype(rows)::value;
+    Thin<T, RN, F, NW, (F == FM ? U : F == 1 ? 4 * U : 2 * U)> p;
+    p.run(a, t, wave, i, g);
+#pragma unroll
+    for (int r = 0; r < RN; r++)
+#pragma unroll
+      for (int f = 0; f < F; f++) lds[wave][r * FM + f][lane] = p.acc[r][f];
+  };
+  if constexpr (FM == 4) {
+    if (live == 1) body(std::integral_constant<int, 1>());
+    else if (live == 2) body(std::integral_constant<int, 2>());
+    else body(std::integral_constant<int, 4>());
+  } else {
+    body(std::integral_constant<int, FM>());
+  }
   __syncthreads();
   for (uint32_t q = wave; q < RN * FM; q += NW) {
     const uint32_t r = q / FM, f = q % FM;
@@ -828,10 +935,11 @@ inline flagcxResult_t launchGrid(const void *kernel, ProductArgs &a, uint32_t bn
   return hipLaunchKernel(kernel, dim3((uint32_t)grid), dim3(threads), argv, 0, s) == hipSuccess ? flagcxSuccess : flagcxUnhandledDeviceError;
 }
 
-template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW, bool DIRECT>
+// SN = 0: guarded
+template <class T, class Out, int BN, int BM, int WN, int WM, int SN, int SM, bool NACROSS, bool MACROSS, bool DW>
 flagcxResult_t launchTiles(ProductArgs a, hipStream_t s) {
   const void *kernel;
-  if constexpr (DIRECT) kernel = reinterpret_cast<const void *>(productDirect<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
+  if constexpr (SN != 0) kernel = reinterpret_cast<const void *>(productDirect<T, Out, BN, BM, WN, WM, SN, SM, NACROSS, MACROSS, DW>);
   else kernel = reinterpret_cast<const void *>(productGuarded<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
   return launchGrid(kernel, a, BN, BM, DW, WN * WM * 64, s);
 }
@@ -848,23 +956,76 @@ inline bool wholeChunks(const void *p, size_t ld, size_t expert, size_t inner, s
   return ((uintptr_t)p & 15) == 0 && ld % e == 0 && expert % e == 0 && inner % e == 0 && ld * es < (1u << 22);
 }
 
+// The tiles of the direct kernels: extent, workgroups that a compute unit holds,
+// and what one slab takes a workgroup, in tenths of a microsecond: alone on its
+// compute unit (`alone`, from calls with fewer workgroups than units: 32 .. 256 rows,
+// n = k = 8192) and with all units full (`full`, from 8192^3).  Large tiles multiply
+// faster, small ones fill the chip with less; the fastest by this account is taken.
+struct TileCost {
+  uint32_t bn, bm, held;
+  float alone, full;
+};
+enum { kTile256, kTile128, kTile256x64, kTile128x64, kTile64, kTiles };
+constexpr TileCost kCost16[kTiles] = {{256, 256, 1, 13.3f, 16.2f}, {128, 128, 2, 8.2f, 4.8f}, {256, 64, 1, 7.2f, 6.2f},
+                                      {128, 64, 2, 4.5f, 2.95f}, {64, 64, 2, 3.4f, 1.94f}};
+constexpr TileCost kCost8[kTiles] = {{256, 256, 1, 20.f, 20.5f}, {128, 128, 2, 11.7f, 6.6f}, {256, 64, 1, 13.2f, 11.4f},
+                                     {128, 64, 2, 9.5f, 4.0f}, {64, 64, 2, 8.6f, 3.1f}};
+
+inline int cheapestTile(const ProductArgs &a, bool dw, const TileCost *cost, int first) {
+  int best = first;
+  float least = 0.f;
+  for (int c = first; c < kTiles; c++) {
+    // an expert's last tile is half full on average, and takes half the time
+    const float m = dw ? (float)((a.m + cost[c].bm - 1) / cost[c].bm) * a.experts
+                       : (a.offsets ? (float)a.rows / cost[c].bm + 0.5f * (a.experts < a.rows ? a.experts : a.rows)
+                                    : (float)((a.rows + cost[c].bm - 1) / cost[c].bm));
+    const float tiles = m * (float)((a.n + cost[c].bn - 1) / cost[c].bn);
+    const uint32_t slots = kUnits * cost[c].held, rounds = (uint32_t)(tiles / slots);
+    const float rest = tiles - (float)rounds * slots;
+    const float deep = (float)(uint32_t)((rest + kUnits - 1) / kUnits) * cost[c].full;   // workgroups sharing a unit in the last round
+    const float t = rounds * cost[c].held * cost[c].full + (rest > 0 ? (deep > cost[c].alone ? deep : cost[c].alone) : 0.f);
+    if (c == first || t < least) {
+      least = t;
+      best = c;
+    }
+  }
+  return best;
+}
+
 template <class T, class Out, bool NACROSS, bool MACROSS, bool DW>
 flagcxResult_t launchShapes(const ProductArgs &a, hipStream_t s) {
   const size_t es = kBytes<T>;
   if constexpr (!NACROSS && !DW) {
-    const uint64_t each = a.rows / (a.experts ? a.experts : 1);
-    if (each <= 4) return launchThin<T, Out, 2, 1, 8, kBytes<T> == 1 ? 2 : 4>(a, s);
-    if (each <= 48) return launchThin<T, Out, 2, 4, 8, 1>(a, s);
+    // Few rows.  (a) up to 8 an expert: 16 at a time, 32 columns a workgroup, or 16
+    // where that leaves units without one (one row, n = k = 4096: 12.2 -> 8.3 us);
+    // eight wavefronts share the reduction, for e4m3 four (16 rows, 8192 x 8192: 19.1
+    // -> 17.0 us; bf16 31.3 -> 28.5 us the other way).  (b) up to 32 rows of one
+    // expert, 64 in e4m3 (35 us against 55 with tiles), or 12 an expert (8 rows each of
+    // 32 experts, 4096 x 4096: 202 us against 262 with tiles; 32 each: 338 against 265).
+    // The lanes' offsets have 31 bits.
+    const bool near = a.ldn * es < (1u << 24) && a.ldm * es < (1u << 24) && a.ldsm < (1u << 22) &&
+                      a.ldsn * (a.n / FX_SCALE_GROUP + 1) < (1u << 28) && (uint64_t)a.k * es < (1u << 30);
+    const uint64_t each = a.rows / a.experts, most = a.experts == 1 ? (es == 1 ? 64 : 32) : 12;
+    const uint64_t m = a.offsets ? a.rows / 16 + (a.experts < a.rows ? a.experts : a.rows) : (a.rows + 15) / 16;
+    const bool wide = m * ((a.n + 31) / 32) >= kUnits;
+    constexpr int NW = kBytes<T> == 1 ? 4 : 8;
+    if (near && each <= 8) return wide ? launchThin<T, Out, 2, 1, NW, 2>(a, s) : launchThin<T, Out, 1, 1, NW, 2>(a, s);
+    if (near && each <= 16 && a.experts == 1) return wide ? launchThin<T, Out, 2, 1, NW, 2>(a, s) : launchThin<T, Out, 1, 1, NW, 2>(a, s);
+    if (near && each <= most) return launchThin<T, Out, 2, 4, 4, 1>(a, s);
   }
   const bool direct = wholeChunks(a.pn, a.ldn, a.expertN, NACROSS ? a.n : a.k, es) &&
                       wholeChunks(a.pm, a.ldm, 0, MACROSS ? a.m : a.k, es);
-  if (!direct) return launchTiles<T, Out, 128, 128, 2, 2, NACROSS, MACROSS, DW, false>(a, s);
-  // Tiles of 256 x 256 when they fill the 256 compute units, else of 128 x 128.
-  const uint64_t big = DW ? (uint64_t)a.experts * ((a.m + 255) / 256) * ((a.n + 255) / 256)
-                          : ((uint64_t)a.rows / 256 + a.experts / 2) * ((a.n + 255) / 256);
-  if constexpr (!__is_same(T, E4m3Exact))      // widened operands leave no registers for the large tile
-    if (big >= 192) return launchTiles<T, Out, 256, 256, 4, 2, NACROSS, MACROSS, DW, true>(a, s);
-  return launchTiles<T, Out, 128, 128, 2, 2, NACROSS, MACROSS, DW, true>(a, s);
+  if (!direct) return launchTiles<T, Out, 128, 128, 2, 2, 0, 0, NACROSS, MACROSS, DW>(a, s);
+  // widened e4m3 operands leave no registers for the largest tile
+  constexpr bool kLargest = !__is_same(T, E4m3Exact);
+  switch (cheapestTile(a, DW, es == 1 ? kCost8 : kCost16, kLargest ? kTile256 : kTile128)) {
+    case kTile256:
+      if constexpr (kLargest) return launchTiles<T, Out, 256, 256, 4, 2, kBytes<T> == 1 ? 2 : 3, 2, NACROSS, MACROSS, DW>(a, s);
+    case kTile128: return launchTiles<T, Out, 128, 128, 2, 2, 2, 2, NACROSS, MACROSS, DW>(a, s);
+    case kTile256x64: return launchTiles<T, Out, 256, 64, 4, 1, 3, 3, NACROSS, MACROSS, DW>(a, s);
+    case kTile128x64: return launchTiles<T, Out, 128, 64, 2, 2, 3, 3, NACROSS, MACROSS, DW>(a, s);
+    default: return launchTiles<T, Out, 64, 64, 1, 2, 4, 4, NACROSS, MACROSS, DW>(a, s);
+  }
 }
 
 template <class T, class Out>

@@ -83,6 +83,15 @@ def test_ragged_products(dev, nk, rows, experts, n, k):
 
 
 @pytest.mark.parametrize("nk", [True, False])
+@pytest.mark.parametrize("rows,experts,n,k", [(40, 1, 520, 1096), (100, 1, 2056, 264), (250, 1, 3080, 136), (600, 1, 1032, 72),
+                                              (1000, 20, 1288, 264), (1900, 32, 2056, 136), (4000, 30, 1032, 72)])
+def test_sizes_between_few_rows_and_full_tiles(dev, nk, rows, experts, n, k):
+    """Where the tile's shape depends on how many tiles there are."""
+    rng = np.random.default_rng(n)
+    run(dev, N.DT_BF16, rows, n, k, None if experts == 1 else ragged(rows, experts, rng), nk=nk, seed=k)
+
+
+@pytest.mark.parametrize("nk", [True, False])
 def test_strides_and_alignment(dev, nk):
     rng = np.random.default_rng(3)
     for pad, shift in ((1, 0), (8, 0), (0, 1), (3, 1), (8, 4)):
@@ -257,6 +266,14 @@ def test_e4m3_ragged_products(dev, rows, experts, n, k):
         o = ragged(rows, experts, rng)
         print(out, rows, experts, n, k, o.tolist()[:20], flush=True)
         run8(dev, rows, n, k, o, out, seed=rows)
+
+
+@pytest.mark.parametrize("rows,experts,n,k", [(40, 1, 528, 1104), (100, 1, 2064, 272), (250, 1, 3088, 144), (600, 1, 1040, 80),
+                                              (1000, 20, 1296, 272), (1900, 32, 2064, 144), (4000, 30, 1040, 272)])
+def test_e4m3_sizes_between_few_rows_and_full_tiles(dev, rows, experts, n, k):
+    rng = np.random.default_rng(n)
+    for out in (N.DT_BF16, N.DT_FP32):
+        run8(dev, rows, n, k, None if experts == 1 else ragged(rows, experts, rng), out, seed=k)
 
 
 def test_e4m3_strides_and_alignment(dev):
