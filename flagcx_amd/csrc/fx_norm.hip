@@ -1,12 +1,13 @@
 // k-way sum + residual + root-mean-square norm (fx_reduce_norm) and its gradients
 // (fx_reduce_norm_grad).
 //
-// A row of C columns is held in the registers of TPR threads, V octets each
-// (octet i * TPR + t belongs to thread t, so 16 neighbouring lanes hold one scale
-// group of 128 columns): inputs are read once, the row's sum of squares is
-// reduced over the threads, and the results leave from the same registers.  The
-// arithmetic is a few operations per element; HBM bounds it.  Rows longer than
-// kHeld columns are read twice (the second pass mostly from the caches).
+// A row of C columns is held in the registers of its threads, V octets each (octet
+// i * threads + t belongs to thread t, so 16 neighbouring lanes hold one scale group
+// of 128 columns): inputs are read once, the row's sum of squares is reduced over
+// the threads, and the results leave from the same registers.  The arithmetic is a
+// few operations per element; HBM bounds it.  Rows of up to 64 V octets are a
+// wavefront's, four to a workgroup; longer ones a workgroup's, with as many
+// wavefronts as they need; rows longer than the registers hold are read twice.
 #include "flagcx_amd/fx_kernels.h"
 #include "flagcx_amd/fx_model.h"
 #include "fx_vec.hpp"
@@ -44,7 +45,7 @@ __device__ __forceinline__ float blockSum(float x, float *lds, uint32_t nWaves) 
 
 // The octet's sum over all inputs, left to right.  B inputs are loaded before the
 // first is used.
-template <class T, int V, int B>
+template <class T, int V, int B, bool APART = false>
 __device__ __forceinline__ void sumInputs(const NormArgs &a, uint32_t row, const uint32_t (&c)[V], float (&f)[V][8]) {
 #pragma unroll
   for (int i = 0; i < V; i++)
@@ -57,12 +58,14 @@ __device__ __forceinline__ void sumInputs(const NormArgs &a, uint32_t row, const
       if (p0 + b < a.n) {
         const T *r = (const T *)a.in[p0 + b] + (size_t)row * (p0 + b < a.k ? a.ldIn : a.ldRes);
 #pragma unroll
-        for (int i = 0; i < V; i++) v[b][i] = loadOctet(r, c[i], a.cols);
+        for (int i = 0; i < V; i++) v[b][i] = loadOctet<false, APART>(r, c[i], a.cols);
       }
 #pragma unroll
     for (int b = 0; b < B; b++)
       if (p0 + b < a.n) {
         const bool first = p0 + b == 0;       // 0 + x would turn -0 into +0
+#pragma unroll
+        for (int i = 0; i < V; i++) settle<APART>(v[b][i], c[i], a.cols);
 #pragma unroll
         for (int i = 0; i < V; i++)
 #pragma unroll
@@ -77,23 +80,25 @@ __device__ __forceinline__ void weights(const NormArgs &a, uint32_t c, float (&w
 #pragma unroll
     for (int j = 0; j < 8; j++) w[j] = 1.f;
   } else if (sizeof(T) == 4 || a.weightF32) {
-    const Octet<float> o = loadOctet((const float *)a.weight, c, a.cols);
+    Octet<float> o = loadOctet((const float *)a.weight, c, a.cols);
+    settle(o, c, a.cols);
 #pragma unroll
     for (int j = 0; j < 8; j++) w[j] = o.get(j);
   } else {
-    const Octet<T> o = loadOctet((const T *)a.weight, c, a.cols);
+    Octet<T> o = loadOctet((const T *)a.weight, c, a.cols);
+    settle(o, c, a.cols);
 #pragma unroll
     for (int j = 0; j < 8; j++) w[j] = o.get(j);
   }
 }
 
-template <class T, bool QUANT>
+template <class T, bool QUANT, bool STREAM>
 __device__ __forceinline__ void finishOctet(const NormArgs &a, uint32_t row, uint32_t c, const float (&f)[8], float r) {
   float w[8], y[8];
   weights<T>(a, c, w);
 #pragma unroll
   for (int j = 0; j < 8; j++) y[j] = f[j] * r * w[j];
-  if (a.total) storeOctet((T *)a.total + (size_t)row * a.ldTotal, c, a.cols, f);
+  if (a.total) storeOctet<STREAM>((T *)a.total + (size_t)row * a.ldTotal, c, a.cols, f);
   if constexpr (QUANT) {
     // The largest magnitude as an integer: NaN > infinity > finite, so a NaN gets through.
     uint32_t m = 0;
@@ -113,38 +118,38 @@ __device__ __forceinline__ void finishOctet(const NormArgs &a, uint32_t row, uin
     const float inv = 1.f / scale;
 #pragma unroll
     for (int j = 0; j < 8; j++) y[j] *= inv;
-    storeE4m3((uint8_t *)a.out + (size_t)row * a.ldOut, c, a.cols, y);
+    storeE4m3<STREAM>((uint8_t *)a.out + (size_t)row * a.ldOut, c, a.cols, y);
     if ((threadIdx.x & 15) == 0 && c < a.cols) a.scale[(size_t)row * a.ldScale + c / FX_SCALE_GROUP] = scale;
   } else {
-    storeOctet((T *)a.out + (size_t)row * a.ldOut, c, a.cols, y);
+    storeOctet<STREAM>((T *)a.out + (size_t)row * a.ldOut, c, a.cols, y);
   }
 }
 
-// One row per TPR threads; with TPR = 64 a workgroup of 256 takes four rows, one per wavefront.
-template <class T, int TPR, int V, bool QUANT>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) normRows(NormArgs a) {
-  constexpr uint32_t kPer = TPR < 256 ? 256 / TPR : 1;
+template <class T, int V, bool WAVE, bool QUANT, bool STREAM>
+__global__ void __launch_bounds__(WAVE ? 256 : 1024) normRows(NormArgs a) {
   __shared__ float lds[16];
-  const uint32_t row = blockIdx.x * kPer + threadIdx.x / TPR;
-  if (row >= a.rows) return;                  // whole wavefronts leave; kPer > 1 has no barrier
+  const uint32_t threads = WAVE ? 64 : blockDim.x, t = WAVE ? threadIdx.x & 63 : threadIdx.x;
+  const uint32_t row = WAVE ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (row >= a.rows) return;                  // whole wavefronts leave, and there is no barrier then
   uint32_t c[V];
 #pragma unroll
-  for (int i = 0; i < V; i++) c[i] = (i * TPR + threadIdx.x % TPR) * 8;
+  for (int i = 0; i < V; i++) c[i] = (i * threads + t) * 8;
   float f[V][8];
-  sumInputs<T, V, (V == 1 ? 8 : V == 2 ? 4 : 2)>(a, row, c, f);
+  sumInputs<T, V, (V == 1 ? (sizeof(T) == 4 ? 8 : 16) : V == 2 ? 4 : 2)>(a, row, c, f);
   float q = 0.f;
 #pragma unroll
   for (int i = 0; i < V; i++)
 #pragma unroll
     for (int j = 0; j < 8; j++) q = __builtin_fmaf(f[i][j], f[i][j], q);
-  q = blockSum(q, lds, TPR / 64);
+  q = blockSum(q, lds, threads / 64);
   const float r = 1.f / sqrtf(q / (float)a.cols + a.eps);
 #pragma unroll
-  for (int i = 0; i < V; i++) finishOctet<T, QUANT>(a, row, c[i], f[i], r);
+  for (int i = 0; i < V; i++) finishOctet<T, QUANT, STREAM>(a, row, c[i], f[i], r);
 }
 
 // Rows wider than the registers hold: the sum is formed twice.  Every element is
-// read and written by one thread in the second pass, so exact aliasing is safe.
+// read and written by one thread in the second pass, so exact aliasing is safe (and
+// the octet that the row ends in must not be read together with its neighbour).
 template <class T, bool QUANT>
 __global__ void __launch_bounds__(1024) normLongRows(NormArgs a) {
   __shared__ float lds[16];
@@ -163,8 +168,8 @@ __global__ void __launch_bounds__(1024) normLongRows(NormArgs a) {
   for (uint32_t s = 0; s < steps; s++) {
     const uint32_t c[1] = {(s * 1024 + threadIdx.x) * 8};
     float f[1][8];
-    sumInputs<T, 1, 8>(a, row, c, f);
-    finishOctet<T, QUANT>(a, row, c[0], f[0], r);
+    sumInputs<T, 1, 8, true>(a, row, c, f);
+    finishOctet<T, QUANT, true>(a, row, c[0], f[0], r);
   }
 }
 
@@ -173,7 +178,8 @@ __global__ void __launch_bounds__(1024) normLongRows(NormArgs a) {
 struct NormGradArgs {
   const void *dy, *x, *dtotal, *weight;
   void *dx;
-  float *partial;                             // [gridDim.x * rows at a time][cols] sums of dweight, or NULL
+  float *partial;                             // sums of dweight, one row of ldPartial floats per part, or NULL
+  uint32_t ldPartial;                         // columns rounded up to 32
   float *rms;                                 // long rows: 1 / rms per row for the column kernel
   size_t ldDy, ldX, ldDtotal, ldDx;
   uint32_t rows, cols;
@@ -190,41 +196,58 @@ __device__ __forceinline__ void gradWeights(const NormGradArgs &a, uint32_t c, f
   weights<T>(n, c, w);
 }
 
-template <class T, int V>
+template <class T, int V, bool STREAM, bool APART = false>
 struct GradRow {
   Octet<T> x[V], dy[V], dt[V];
   __device__ __forceinline__ void load(const NormGradArgs &a, uint32_t row, const uint32_t (&c)[V]) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      x[i] = loadOctet((const T *)a.x + (size_t)row * a.ldX, c[i], a.cols);
-      dy[i] = loadOctet((const T *)a.dy + (size_t)row * a.ldDy, c[i], a.cols);
+      x[i] = loadOctet<STREAM, APART>((const T *)a.x + (size_t)row * a.ldX, c[i], a.cols);
+      dy[i] = loadOctet<STREAM, APART>((const T *)a.dy + (size_t)row * a.ldDy, c[i], a.cols);
     }
     if (a.dtotal && a.dx)
 #pragma unroll
-      for (int i = 0; i < V; i++) dt[i] = loadOctet((const T *)a.dtotal + (size_t)row * a.ldDtotal, c[i], a.cols);
+      for (int i = 0; i < V; i++) dt[i] = loadOctet<STREAM, APART>((const T *)a.dtotal + (size_t)row * a.ldDtotal, c[i], a.cols);
+  }
+  __device__ __forceinline__ void ready(const NormGradArgs &a, const uint32_t (&c)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      settle<APART>(x[i], c[i], a.cols);
+      settle<APART>(dy[i], c[i], a.cols);
+      if (a.dtotal && a.dx) settle<APART>(dt[i], c[i], a.cols);
+    }
   }
 };
 
-// A workgroup walks rows blockIdx.x, blockIdx.x + gridDim.x, ... (per TPR threads),
-// keeps its columns' share of dweight in registers and stores it once at the end.
-template <class T, int TPR, int V>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) normGradRows(NormGradArgs a) {
-  constexpr uint32_t kPer = TPR < 256 ? 256 / TPR : 1;
-  __shared__ float lds[2][16];
-  const uint32_t lane = threadIdx.x % TPR, slot = blockIdx.x * kPer + threadIdx.x / TPR;
-  uint32_t c[V];
+// Row r, r + gridDim.x, ... of a workgroup (WAVE: of each of its four wavefronts):
+// the next row is loaded while this one is reduced (a workgroup of 1024 has no
+// registers for that), and the columns' share of dweight stays in registers until the
+// end.
+template <class T, int V, bool WAVE, int THREADS, bool STREAM>
+__global__ void __launch_bounds__(THREADS) normGradRows(NormGradArgs a) {
+  constexpr bool kAhead = THREADS <= 512;
+  __shared__ float lds[2][2][16];
+  __shared__ float joined[WAVE ? 3 : 1][WAVE ? 64 * V * 8 : 1];
+  const uint32_t threads = WAVE ? 64 : blockDim.x, t = WAVE ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6;
+  const uint32_t step = gridDim.x * (WAVE ? 4 : 1);
+  uint32_t c[V], row = WAVE ? blockIdx.x * 4 + wave : blockIdx.x;
   float w[V][8], dw[V][8];
 #pragma unroll
+  for (int i = 0; i < V; i++) c[i] = (i * threads + t) * 8;
+  GradRow<T, V, STREAM> next;
+  if (kAhead && row < a.rows) next.load(a, row, c);
+#pragma unroll
   for (int i = 0; i < V; i++) {
-    c[i] = (i * TPR + lane) * 8;
     gradWeights<T>(a, c[i], w[i]);
 #pragma unroll
     for (int j = 0; j < 8; j++) dw[i][j] = 0.f;
   }
   const float invC = 1.f / (float)a.cols;
-  for (uint32_t row = slot; row < a.rows; row += gridDim.x * kPer) {
-    GradRow<T, V> g;
-    g.load(a, row, c);
+  for (uint32_t turn = 0; row < a.rows; row += step, turn ^= 1) {
+    if (!kAhead) next.load(a, row, c);
+    GradRow<T, V, STREAM> g = next;
+    if (kAhead && row + step < a.rows) next.load(a, row + step, c);
+    g.ready(a, c);
     float q = 0.f, m = 0.f;
 #pragma unroll
     for (int i = 0; i < V; i++)
@@ -236,18 +259,16 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) normGradRows(NormGradAr
       }
     q = waveSum(q);
     m = waveSum(m);
-    if constexpr (TPR > 64) {
-      __syncthreads();                        // the row before has been read by everybody
-      if ((threadIdx.x & 63) == 0) {
-        lds[0][threadIdx.x >> 6] = q;
-        lds[1][threadIdx.x >> 6] = m;
+    if constexpr (!WAVE) {
+      if (t % 64 == 0) {                      // two sets in turn: one barrier a row
+        lds[turn][0][wave] = q;
+        lds[turn][1][wave] = m;
       }
       __syncthreads();
       q = m = 0.f;
-#pragma unroll
-      for (int s = 0; s < TPR / 64; s++) {
-        q += lds[0][s];
-        m += lds[1][s];
+      for (uint32_t s = 0; s < threads / 64; s++) {
+        q += lds[turn][0][s];
+        m += lds[turn][1][s];
       }
     }
     const float r = 1.f / sqrtf(q * invC + a.eps);
@@ -262,12 +283,28 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) normGradRows(NormGradAr
         d[j] = r * __builtin_fmaf(-x, h, dy * w[i][j]);
         if (a.dtotal) d[j] += g.dt[i].get(j);
       }
-      if (a.dx) storeOctet((T *)a.dx + (size_t)row * a.ldDx, c[i], a.cols, d);
+      if (a.dx) storeOctet<STREAM>((T *)a.dx + (size_t)row * a.ldDx, c[i], a.cols, d);
     }
   }
-  if (a.partial)
+  if (!a.partial) return;
+  if constexpr (WAVE) {                       // the four wavefronts' sums, in order
+    if (wave)
 #pragma unroll
-    for (int i = 0; i < V; i++) storeOctet(a.partial + (size_t)slot * a.cols, c[i], a.cols, dw[i]);
+      for (int i = 0; i < V; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) joined[wave - 1][c[i] + j] = dw[i][j];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int i = 0; i < V; i++)
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int s = 0; s < 3; s++) dw[i][j] += joined[s][c[i] + j];
+  }
+#pragma unroll
+  for (int i = 0; i < V; i++)
+    if (c[i] < a.ldPartial) storeOctet(a.partial + (size_t)blockIdx.x * a.ldPartial, c[i], a.ldPartial, dw[i]);   // zeros behind the last column
 }
 
 template <class T>
@@ -278,8 +315,9 @@ __global__ void __launch_bounds__(1024) normGradLongRows(NormGradArgs a) {
   float q = 0.f, m = 0.f;
   for (uint32_t s = 0; s < steps; s++) {
     const uint32_t c[1] = {(s * 1024 + threadIdx.x) * 8};
-    GradRow<T, 1> g;
+    GradRow<T, 1, false> g;
     g.load(a, row, c);
+    g.ready(a, c);
     float w[8];
     gradWeights<T>(a, c[0], w);
 #pragma unroll
@@ -298,8 +336,9 @@ __global__ void __launch_bounds__(1024) normGradLongRows(NormGradArgs a) {
   if (!a.dx) return;
   for (uint32_t s = 0; s < steps; s++) {
     const uint32_t c[1] = {(s * 1024 + threadIdx.x) * 8};
-    GradRow<T, 1> g;
+    GradRow<T, 1, false, true> g;
     g.load(a, row, c);
+    g.ready(a, c);
     float w[8], d[8];
     gradWeights<T>(a, c[0], w);
 #pragma unroll
@@ -318,43 +357,46 @@ __global__ void __launch_bounds__(256) normGradLongColumns(NormGradArgs a) {
   const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * 8;
   float dw[8] = {};
   for (uint32_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-    const Octet<T> x = loadOctet((const T *)a.x + (size_t)row * a.ldX, c, a.cols);
-    const Octet<T> dy = loadOctet((const T *)a.dy + (size_t)row * a.ldDy, c, a.cols);
+    Octet<T> x = loadOctet((const T *)a.x + (size_t)row * a.ldX, c, a.cols);
+    Octet<T> dy = loadOctet((const T *)a.dy + (size_t)row * a.ldDy, c, a.cols);
+    settle(x, c, a.cols);
+    settle(dy, c, a.cols);
     const float r = a.rms[row];
 #pragma unroll
     for (int j = 0; j < 8; j++) dw[j] = __builtin_fmaf(dy.get(j), x.get(j) * r, dw[j]);
   }
-  storeOctet(a.partial + (size_t)blockIdx.y * a.cols, c, a.cols, dw);
+  if (c < a.ldPartial) storeOctet(a.partial + (size_t)blockIdx.y * a.ldPartial, c, a.ldPartial, dw);
 }
 
-// dweight = sum of `n` rows of partial sums, in a fixed order: 16 groups of rows
-// per 64 columns, joined through LDS.
+// dweight = sum of `n` rows of partial sums, in a fixed order: 32 columns a
+// workgroup, every 32nd row to each of 32 groups of eight lanes, eight rows on their
+// way at a time; the groups meet in LDS.
 template <class W>
-__global__ void __launch_bounds__(256) normGradJoin(const float *partial, uint32_t n, uint32_t cols, W *dweight) {
-  __shared__ float lds[16][64];
-  const uint32_t part = threadIdx.x >> 4, c = blockIdx.x * 64 + (threadIdx.x & 15) * 4;
-  float s[4] = {};
-  for (uint32_t r = part; r < n; r += 16) {
-    const float *p = partial + (size_t)r * cols;
-    if (c + 4 <= cols) {
-      typedef float f32x4_anywhere __attribute__((ext_vector_type(4), aligned(4)));
-      const f32x4_anywhere v = *reinterpret_cast<const f32x4_anywhere *>(p + c);
+__global__ void __launch_bounds__(256) normGradJoin(const float *partial, uint32_t n, uint32_t ld, uint32_t cols, W *dweight) {
+  __shared__ float lds[32][33];
+  const uint32_t part = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
+  const float *p = partial + blockIdx.x * 32 + c;
+  f32x4 s = {};
+  for (uint32_t r0 = part; r0 < n; r0 += 256) {
+    f32x4 v[8];
 #pragma unroll
-      for (int j = 0; j < 4; j++) s[j] += v[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (c + j < cols) s[j] += p[c + j];
+    for (int u = 0; u < 8; u++) {
+      const uint32_t r = r0 + 32 * u;
+      v[u] = r < n ? *reinterpret_cast<const f32x4 *>(p + (size_t)r * ld) : f32x4{};
     }
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) s[j] += v[u][j];
   }
 #pragma unroll
-  for (int j = 0; j < 4; j++) lds[part][(threadIdx.x & 15) * 4 + j] = s[j];
+  for (int j = 0; j < 4; j++) lds[part][c + j] = s[j];
   __syncthreads();
-  if (threadIdx.x < 64 && blockIdx.x * 64 + threadIdx.x < cols) {
+  if (threadIdx.x < 32 && blockIdx.x * 32 + threadIdx.x < cols) {
     float t = 0.f;
 #pragma unroll
-    for (int p = 0; p < 16; p++) t += lds[p][threadIdx.x];
-    dweight[blockIdx.x * 64 + threadIdx.x] = (W)t;
+    for (int q = 0; q < 32; q++) t += lds[q][threadIdx.x];
+    dweight[blockIdx.x * 32 + threadIdx.x] = (W)t;
   }
 }
 
@@ -384,23 +426,36 @@ flagcxResult_t screenTypes(int dtype, int weightDtype) {
   return flagcxSuccess;
 }
 
-constexpr size_t kMaxExtent = 0x7fffffff;
+constexpr size_t kMaxExtent = 0x7fffffe0;   // also when rounded up to 32
+constexpr uint32_t kFewRows = 512;
+constexpr uint64_t kStreamBytes = 32u << 20, kGradStreamBytes = 128u << 20;
 
+// Wavefronts that hold `octets`, v to a lane, in threads.
+uint32_t threadsFor(uint32_t octets, uint32_t v) { return ((octets + v - 1) / v + 63) / 64 * 64; }
+
+template <class T, bool QUANT, bool STREAM>
+flagcxResult_t launchNormRows(const NormArgs &a, hipStream_t s) {
+  const uint32_t octets = (a.cols + 7) / 8, fours = (a.rows + 3) / 4;
+  if (octets <= 64) return launchShape(normRows<T, 1, true, QUANT, STREAM>, dim3(fours), 256, s, a);
+  // Few rows: one octet to a lane, so that all inputs of a row are on their way at once (one row of 8192 with eight
+  // inputs 8.4 -> 6.4 us).
+  if constexpr (!STREAM)
+    if (octets <= 1024 && a.rows <= kFewRows) return launchShape(normRows<T, 1, false, QUANT, STREAM>, dim3(a.rows), threadsFor(octets, 1), s, a);
+  if (octets <= 128) return launchShape(normRows<T, 2, true, QUANT, STREAM>, dim3(fours), 256, s, a);
+  if (octets <= 512) return launchShape(normRows<T, 2, false, QUANT, STREAM>, dim3(a.rows), threadsFor(octets, 2), s, a);
+  return launchShape(normRows<T, 4, false, QUANT, STREAM>, dim3(a.rows), threadsFor(octets, 4), s, a);
+}
+
+// Results that the dies' L2s (32 MiB) cannot hold are streamed (16384 x 8192, two bf16
+// inputs and the residual to e4m3: 216 -> 208 us; 4096 x 4096, four inputs: 47 -> 45
+// us); smaller ones stay for whoever reads them next.  Loads are left to the caches:
+// streaming them gained 5 % from memory and cost 30 % when the inputs had just been
+// written (1024 x 4096).
 template <class T, bool QUANT>
 flagcxResult_t launchNorm(const NormArgs &a, hipStream_t s) {
-  const uint32_t octets = (a.cols + 7) / 8;
-  auto go = [&](auto kernel, uint32_t tpr) {
-    const uint32_t per = tpr < 256 ? 256 / tpr : 1;
-    return launchShape(kernel, dim3((a.rows + per - 1) / per), tpr < 256 ? 256 : tpr, s, a);
-  };
   if (a.cols > kHeld) return launchShape(normLongRows<T, QUANT>, dim3(a.rows), 1024, s, a);
-  if (octets <= 64) return go(normRows<T, 64, 1, QUANT>, 64);
-  if (octets <= 128) return go(normRows<T, 64, 2, QUANT>, 64);
-  if (octets <= 256) return go(normRows<T, 256, 1, QUANT>, 256);
-  if (octets <= 512) return go(normRows<T, 256, 2, QUANT>, 256);
-  if (octets <= 1024) return go(normRows<T, 256, 4, QUANT>, 256);
-  if (octets <= 2048) return go(normRows<T, 512, 4, QUANT>, 512);
-  return go(normRows<T, 1024, 4, QUANT>, 1024);
+  const uint64_t written = (uint64_t)a.rows * a.cols * ((a.total ? sizeof(T) : 0) + (QUANT ? 1 : sizeof(T)));
+  return written > kStreamBytes ? launchNormRows<T, QUANT, true>(a, s) : launchNormRows<T, QUANT, false>(a, s);
 }
 
 template <class T>
@@ -408,57 +463,42 @@ flagcxResult_t launchNormOut(const NormArgs &a, bool quant, hipStream_t s) {
   return quant ? launchNorm<T, true>(a, s) : launchNorm<T, false>(a, s);
 }
 
-// Rows of partial sums of dweight.  Two workgroups per CU keep the loads busy;
-// fewer when there are fewer rows.
-constexpr uint32_t kGradWgs = 512;
+// Workgroups of the gradients, each with a row of partial sums: one per compute unit
+// (8192 x 8192 bf16: 89 us, with 384 105, with 512 94); fewer when there are fewer rows.
+constexpr uint32_t kGradWgs = 256;
 constexpr uint32_t kLongParts = 64;
+constexpr uint32_t kGradHeld = 1024 * 2 * 8;   // widest row that the gradients hold
 
-struct GradShape {
-  uint32_t tpr, v, wgs, parts;
-};
-GradShape gradShape(size_t rows, size_t cols) {
-  const size_t octets = (cols + 7) / 8;
-  GradShape g;
-  if (octets <= 64) g = {64, 1, 0, 0};
-  else if (octets <= 128) g = {64, 2, 0, 0};
-  else if (octets <= 256) g = {256, 1, 0, 0};
-  else if (octets <= 512) g = {256, 2, 0, 0};
-  else if (octets <= 1024) g = {256, 4, 0, 0};
-  else if (octets <= 2048) g = {512, 4, 0, 0};
-  else g = {1024, 4, 0, 0};
-  const size_t per = g.tpr < 256 ? 256 / g.tpr : 1;
-  const size_t want = (rows + per - 1) / per;
-  g.wgs = (uint32_t)(want < kGradWgs ? want : kGradWgs);
-  g.parts = g.wgs * (uint32_t)per;
-  return g;
+uint32_t partialStride(size_t cols) { return (uint32_t)((cols + 31) / 32 * 32); }
+bool waveRows(size_t cols) { return cols <= 64 * 2 * 8; }
+uint32_t gradParts(size_t rows, size_t cols) {
+  const size_t most = cols > kGradHeld ? kLongParts : kGradWgs;
+  const size_t want = waveRows(cols) ? (rows + 3) / 4 : rows;
+  return (uint32_t)(want < most ? want : most);
 }
 
-template <class T>
-flagcxResult_t launchGradRows(const NormGradArgs &a, const GradShape &g, hipStream_t s) {
-  auto go = [&](auto kernel) { return launchShape(kernel, dim3(g.wgs), g.tpr < 256 ? 256 : g.tpr, s, a); };
-  switch (g.tpr * 8 + g.v) {
-    case 64 * 8 + 1: return go(normGradRows<T, 64, 1>);
-    case 64 * 8 + 2: return go(normGradRows<T, 64, 2>);
-    case 256 * 8 + 1: return go(normGradRows<T, 256, 1>);
-    case 256 * 8 + 2: return go(normGradRows<T, 256, 2>);
-    case 256 * 8 + 4: return go(normGradRows<T, 256, 4>);
-    case 512 * 8 + 4: return go(normGradRows<T, 512, 4>);
-    default: return go(normGradRows<T, 1024, 4>);
-  }
+template <class T, bool STREAM>
+flagcxResult_t launchGradRows(const NormGradArgs &a, uint32_t parts, hipStream_t s) {
+  const uint32_t octets = (a.cols + 7) / 8;
+  if (octets <= 64) return launchShape(normGradRows<T, 1, true, 256, STREAM>, dim3(parts), 256, s, a);
+  if (waveRows(a.cols)) return launchShape(normGradRows<T, 2, true, 256, STREAM>, dim3(parts), 256, s, a);
+  if (octets <= 512) return launchShape(normGradRows<T, 1, false, 512, STREAM>, dim3(parts), threadsFor(octets, 1), s, a);
+  if (octets <= 1024) return launchShape(normGradRows<T, 2, false, 512, STREAM>, dim3(parts), threadsFor(octets, 2), s, a);
+  return launchShape(normGradRows<T, 2, false, 1024, STREAM>, dim3(parts), threadsFor(octets, 2), s, a);
 }
 
 template <class T>
 flagcxResult_t launchGrad(NormGradArgs a, void *dweight, bool weightF32, void *workspace, hipStream_t s) {
-  uint32_t parts = 0;
+  const uint32_t parts = a.rows ? gradParts(a.rows, a.cols) : 0;
   flagcxResult_t rc = flagcxSuccess;
   a.partial = dweight ? (float *)workspace : nullptr;
+  a.ldPartial = partialStride(a.cols);
   a.rms = nullptr;
-  if (a.rows && a.cols > kHeld) {
+  if (a.rows && a.cols > kGradHeld) {
     // The column kernel reads dy and x again, so it goes before the pass that writes dx (which may equal dy):
     // rms first, without dx; then the columns; then dx.
     if (dweight) {
-      parts = a.rows < kLongParts ? a.rows : kLongParts;
-      a.rms = (float *)workspace + (size_t)kLongParts * a.cols;
+      a.rms = (float *)workspace + (size_t)parts * a.ldPartial;
       NormGradArgs b = a;
       b.dx = nullptr;
       rc = launchShape(normGradLongRows<T>, dim3(a.rows), 1024, s, b);
@@ -468,14 +508,16 @@ flagcxResult_t launchGrad(NormGradArgs a, void *dweight, bool weightF32, void *w
     }
     if (a.dx) rc = launchShape(normGradLongRows<T>, dim3(a.rows), 1024, s, a);
   } else if (a.rows) {
-    const GradShape g = gradShape(a.rows, a.cols);
-    parts = g.parts;
-    rc = launchGradRows<T>(a, g, s);
+    // What the memory-side cache cannot keep is streamed both ways (8192 x 4096 bf16: 54 -> 50 us, 8192 x 8192: 107 ->
+    // 95 us).
+    const uint64_t bytes = (uint64_t)a.rows * a.cols * sizeof(T) * (2 + (a.dx ? 1 + (a.dtotal != nullptr) : 0));
+    rc = bytes > kGradStreamBytes ? launchGradRows<T, true>(a, parts, s) : launchGradRows<T, false>(a, parts, s);
   }
   if (rc != flagcxSuccess || !dweight) return rc;
-  const dim3 grid((a.cols + 63) / 64);
-  if (weightF32) return launchShape(normGradJoin<float>, grid, 256, s, (const float *)workspace, parts, a.cols, (float *)dweight);
-  return launchShape(normGradJoin<T>, grid, 256, s, (const float *)workspace, parts, a.cols, (T *)dweight);
+  const dim3 grid(a.ldPartial / 32);
+  if (weightF32)
+    return launchShape(normGradJoin<float>, grid, 256, s, (const float *)workspace, parts, a.ldPartial, a.cols, (float *)dweight);
+  return launchShape(normGradJoin<T>, grid, 256, s, (const float *)workspace, parts, a.ldPartial, a.cols, (T *)dweight);
 }
 
 }  // namespace
@@ -532,8 +574,8 @@ int fx_reduce_norm(void *out, float *scale, void *total, const void *const *in, 
 
 size_t fx_reduce_norm_grad_workspace(size_t rows, size_t cols) {
   if (rows == 0 || cols == 0) return 0;
-  if (cols > kHeld) return ((size_t)kLongParts * cols + rows) * sizeof(float);
-  return (size_t)gradShape(rows, cols).parts * cols * sizeof(float);
+  if (rows > kMaxExtent || cols > kMaxExtent) return 0;
+  return ((size_t)gradParts(rows, cols) * partialStride(cols) + (cols > kGradHeld ? rows : 0)) * sizeof(float);
 }
 
 int fx_reduce_norm_grad(void *dx, void *dweight, const void *dy, const void *x, const void *dtotal, const void *weight,

@@ -49,19 +49,40 @@ struct Octet<float> {
   }
 };
 
-// Octet at columns [c, c + 8) of a row of `cols` elements; columns behind the
-// last read as zero and are not touched.  gfx950 serves 128-bit accesses at any
-// element boundary, so rows of odd length need no path of their own.
-template <class T>
+// STREAM: past the caches.
+template <bool STREAM>
+__device__ __forceinline__ u32x4 loadVec(const u32x4_anywhere *p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+typedef uint32_t u32x2_anywhere __attribute__((ext_vector_type(2), aligned(1)));
+template <bool STREAM>
+__device__ __forceinline__ void storeVec(u32x4_anywhere *p, u32x4 v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+template <bool STREAM>
+__device__ __forceinline__ void storeVec(u32x2_anywhere *p, u32x2_anywhere v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+// Octet at columns [c, c + 8) of a row of `cols` elements.  gfx950 serves 128-bit
+// accesses at any element boundary, so rows of odd length need no path of their own:
+// an octet that the row ends in is loaded from the row's last eight elements (no
+// branch around the load, nothing behind the row touched) and shifted into place by
+// settle(), which is called where the octet is first used; columns behind the last
+// are zero then.  APART: element by element instead, for passes that have written
+// other columns of the row already.
+template <bool STREAM = false, bool APART = false, class T>
 __device__ __forceinline__ Octet<T> loadOctet(const T *row, uint32_t c, uint32_t cols) {
   Octet<T> o = {};
-  if (c + 8 <= cols) {
-    const u32x4_anywhere *p = reinterpret_cast<const u32x4_anywhere *>(row + c);
+  if (APART ? c + 8 <= cols : cols >= 8) {
+    const u32x4_anywhere *p = reinterpret_cast<const u32x4_anywhere *>(row + (c < cols - 8 ? c : cols - 8));
     if constexpr (sizeof(T) == 4) {
-      o.v[0] = p[0];
-      o.v[1] = p[1];
+      o.v[0] = loadVec<STREAM>(p);
+      o.v[1] = loadVec<STREAM>(p + 1);
     } else {
-      o.v = p[0];
+      o.v = loadVec<STREAM>(p);
     }
   } else if (c < cols) {
     float f[8];
@@ -72,17 +93,51 @@ __device__ __forceinline__ Octet<T> loadOctet(const T *row, uint32_t c, uint32_t
   return o;
 }
 
-template <class T>
+template <bool APART = false, class T>
+__device__ __forceinline__ void settle(Octet<T> &o, uint32_t c, uint32_t cols) {
+  if (APART || cols < 8 || c + 8 <= cols) return;
+  const uint32_t s = c + 8 - cols;            // elements to drop in front
+  if (s >= 8) {
+    o = Octet<T>{};
+    return;
+  }
+  if constexpr (sizeof(T) == 4) {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) w[j] = o.v[j >> 2][j & 3];
+#pragma unroll
+    for (int b = 1; b < 8; b <<= 1)
+#pragma unroll
+      for (int j = 0; j < 8; j++) w[j] = (s & b) ? (j + b < 8 ? w[j + b] : 0u) : w[j];
+#pragma unroll
+    for (int j = 0; j < 8; j++) o.v[j >> 2][j & 3] = w[j];
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = o.v[j];
+#pragma unroll
+    for (int b = 1; b < 4; b <<= 1)
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] = (s >> 1 & b) ? (j + b < 4 ? w[j + b] : 0u) : w[j];
+    if (s & 1)
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] = w[j] >> 16 | (j < 3 ? w[j < 3 ? j + 1 : 3] << 16 : 0u);
+#pragma unroll
+    for (int j = 0; j < 4; j++) o.v[j] = w[j];
+  }
+}
+
+template <bool STREAM = false, class T>
 __device__ __forceinline__ void storeOctet(T *row, uint32_t c, uint32_t cols, const float (&f)[8]) {
   if (c + 8 <= cols) {
     Octet<T> o;
     o.set(f);
     u32x4_anywhere *p = reinterpret_cast<u32x4_anywhere *>(row + c);
     if constexpr (sizeof(T) == 4) {
-      p[0] = o.v[0];
-      p[1] = o.v[1];
+      storeVec<STREAM>(p, o.v[0]);
+      storeVec<STREAM>(p + 1, o.v[1]);
     } else {
-      p[0] = o.v;
+      storeVec<STREAM>(p, o.v);
     }
   } else if (c < cols) {
 #pragma unroll
@@ -92,6 +147,7 @@ __device__ __forceinline__ void storeOctet(T *row, uint32_t c, uint32_t cols, co
 }
 
 // Eight floats as e4m3 codes (round to nearest even), columns behind the last left alone.
+template <bool STREAM>
 __device__ __forceinline__ void storeE4m3(uint8_t *row, uint32_t c, uint32_t cols, const float (&f)[8]) {
   uint32_t w[2];
 #pragma unroll
@@ -101,11 +157,10 @@ __device__ __forceinline__ void storeE4m3(uint8_t *row, uint32_t c, uint32_t col
     w[h] = (uint32_t)q;
   }
   if (c + 8 <= cols) {
-    typedef uint32_t u32x2_anywhere __attribute__((ext_vector_type(2), aligned(1)));
     u32x2_anywhere v;
     v[0] = w[0];
     v[1] = w[1];
-    *reinterpret_cast<u32x2_anywhere *>(row + c) = v;
+    storeVec<STREAM>(reinterpret_cast<u32x2_anywhere *>(row + c), v);
   } else if (c < cols) {
 #pragma unroll
     for (int j = 0; j < 8; j++)

@@ -119,7 +119,7 @@ def test_norm_strides_and_alignment(dev, name, quant, weight):
 
 
 @pytest.mark.parametrize("alias", ["total=residual", "total=in", "out=in"])
-@pytest.mark.parametrize("cols", [100, 2000, 9000, 35000])
+@pytest.mark.parametrize("cols", [3, 100, 515, 2000, 2052, 9000, 35000, 32772, 40963])
 def test_norm_in_place(dev, alias, cols):
     run_norm(dev, N.DT_BF16, 6, cols, 3, alias=alias, seed=cols)
     run_norm(dev, N.DT_FP32, 2, cols, 2, alias=alias, seed=cols, pad=4)
@@ -208,7 +208,7 @@ def test_norm_gradient_rows(dev, rows):
 
 
 @pytest.mark.parametrize("name", TYPES)
-@pytest.mark.parametrize("cols", [200, 3000, 33010])
+@pytest.mark.parametrize("cols", [3, 200, 516, 3000, 4099, 16381, 32772, 33010])
 def test_norm_gradient_strides_aliases_and_parts(dev, name, cols):
     t = TYPES[name]
     run_grad(dev, t, 6, cols, pad=3, shift=1, seed=cols)
