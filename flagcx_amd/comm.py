@@ -16,6 +16,7 @@ or ``borrow_stream`` around a foreign hipStream_t).  A failing call raises
 ``N.FlagcxError`` carrying the flagcxResult_t code and the library's text for it.
 """
 import ctypes as C
+import functools
 
 from . import _native as N
 from .adaptor import load_plugin
@@ -31,6 +32,7 @@ _DTYPE_BY_NAME = {"int8": N.DT_INT8, "uint8": N.DT_UINT8, "int32": N.DT_INT32, "
 _OP_BY_NAME = {"SUM": N.OP_SUM, "PRODUCT": N.OP_PROD, "MAX": N.OP_MAX, "MIN": N.OP_MIN, "AVG": N.OP_AVG}
 
 
+@functools.lru_cache(maxsize=64)
 def dtype_code(torch_dtype):
     """FlagCX datatype of a torch dtype (``torch.bfloat16`` -> 9)."""
     name = str(torch_dtype).rsplit(".", 1)[-1]
