@@ -325,6 +325,67 @@ __device__ __forceinline__ void storeRun(Out *p, uint32_t c, uint32_t cols, cons
   }
 }
 
+// Four fragments side by side, of each of which a lane of group g holds columns
+// 4 g .. 4 g + 3: turned over the four groups, so that group g holds all sixteen
+// columns of fragment g and a row's 64 leave in pieces of 32 bytes or more.
+__device__ __forceinline__ void turn4(uint32_t (&w)[4]) {
+  auto swap16 = [](uint32_t &x, uint32_t &y) {   // odd groups of x against even groups of y
+    const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    x = r[0];
+    y = r[1];
+  };
+  auto swap32 = [](uint32_t &x, uint32_t &y) {   // groups 2, 3 of x against 0, 1 of y
+    const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    x = r[0];
+    y = r[1];
+  };
+  swap16(w[0], w[1]);
+  swap16(w[2], w[3]);
+  swap32(w[0], w[2]);
+  swap32(w[1], w[3]);
+  // now w[0], w[1], w[2], w[3]: the first, second, third and last four columns
+}
+template <class Out>
+__device__ __forceinline__ void storeTurned(Out *row, uint32_t c, uint32_t cols, const f32x4 (&part)[4]) {
+  float v[16];
+  if constexpr (sizeof(Out) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      uint32_t w[4];
+#pragma unroll
+      for (int f = 0; f < 4; f++) {
+        const float x = part[f][j];           // a value: __builtin_bit_cast of a vector's element takes the first
+        w[f] = __builtin_bit_cast(uint32_t, x);
+      }
+      turn4(w);
+#pragma unroll
+      for (int h = 0; h < 4; h++) v[4 * h + j] = __builtin_bit_cast(float, w[h]);
+    }
+    storeRun(row, c, cols, v);
+  } else {
+    uint32_t out[8];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      uint32_t w[4];
+#pragma unroll
+      for (int f = 0; f < 4; f++)
+        w[f] = (uint32_t)__builtin_bit_cast(uint16_t, (Out)part[f][2 * j]) |
+               ((uint32_t)__builtin_bit_cast(uint16_t, (Out)part[f][2 * j + 1]) << 16);
+      turn4(w);
+#pragma unroll
+      for (int h = 0; h < 4; h++) out[2 * h + j] = w[h];
+    }
+    if (c + 16 <= cols) {
+      *reinterpret_cast<u32x4_anywhere *>(row + c) = u32x4{out[0], out[1], out[2], out[3]};
+      *reinterpret_cast<u32x4_anywhere *>(row + c + 8) = u32x4{out[4], out[5], out[6], out[7]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (c + j < cols) reinterpret_cast<uint16_t *>(row)[c + j] = (uint16_t)(out[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+
 // ---------------------------------------------------------------- the kernel
 
 // WN x WM wavefronts, each with a (BN / WN) x (BM / WM) part of the tile.
@@ -402,13 +463,14 @@ struct Product {
 #pragma unroll
     for (int q = 0; q < FM; q++) {
       const uint32_t m = t.m0 + wm + 16 * q + i;
-      if (m >= t.mEnd) continue;
+      const bool live = m < t.mEnd;
+      if (!NACROSS && !live) continue;        // the across form exchanges between lanes first
       Out *row = y + (size_t)m * a.ldy;
       if constexpr (NACROSS) {
 #pragma unroll
-        for (int f = 0; f < FN; f++) {
-          const float v[4] = {acc[f][q][0], acc[f][q][1], acc[f][q][2], acc[f][q][3]};
-          storeRun(row, t.n0 + wn + 16 * f + 4 * g, a.n, v);
+        for (int b = 0; b < FN / 4; b++) {
+          const f32x4 part[4] = {acc[4 * b][q], acc[4 * b + 1][q], acc[4 * b + 2][q], acc[4 * b + 3][q]};
+          storeTurned<Out>(row, live ? t.n0 + wn + 64 * b + 16 * g : a.n, a.n, part);
         }
       } else {
 #pragma unroll
@@ -557,6 +619,14 @@ struct DirectScales {
   }
 };
 
+// TOUCH: the largest e4m3 tile has LDS for two buffers only, and one slab's time is
+// less than memory takes under load.  Two wavefronts also touch lines of a slab
+// further on, four bytes of each that nobody reads, which brings them into the die's
+// cache; neighbouring tiles share a slab's lines out among them.  Loads return in
+// order; the wait for a slab leaves the last touch out, so it has two slabs' time.
+// (8192^3 from memory 633 -> 579 us; where few tiles share weights it gains nothing.)
+constexpr uint32_t kTouchAhead = 4;
+
 // The slabs as a pipeline.  A slab is multiplied in phases; the fragments of
 // the next phase are read from LDS while this one's are multiplied.  In front of
 // the last phase all of a slab's fragments are in registers: there the wavefronts
@@ -571,13 +641,14 @@ struct DirectScales {
 // accumulators two products later, in the shadow of the matrix instructions.
 #define FX_FENCE() __builtin_amdgcn_sched_barrier(0)
 
-template <class T, class Out, int BN, int BM, int WN, int WM, int SN, int SM, bool NACROSS, bool MACROSS, bool DW>
+template <class T, class Out, int BN, int BM, int WN, int WM, int SN, int SM, bool NACROSS, bool MACROSS, bool DW, bool TOUCH>
 __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
   using P = Product<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>;
   constexpr uint32_t kStageM = P::kLdsM + (P::kScaled ? P::kThreads * 4 : 0), kLds = SN * P::kLdsN + SM * kStageM;
-  constexpr int kLoadsN = P::N::kLoads, kLoadsM = P::M::kLoads + P::kScaled;   // per thread and slab
+  constexpr int kLoadsN = P::N::kLoads + TOUCH, kLoadsM = P::M::kLoads + P::kScaled;   // per thread and slab
   static_assert(BM <= P::kThreads && SN >= SM && SM >= 2, "a thread per row's scale");
-  __shared__ __attribute__((aligned(1024))) char lds[kLds];
+  static_assert(!TOUCH || (!NACROSS && !MACROSS && BN == 256 && BM == 256 && SN == 2), "lines as rows");
+  __shared__ __attribute__((aligned(1024))) char lds[kLds + (TOUCH ? 256 : 0)];
   typedef __attribute__((address_space(3))) char *ldsPtr;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(ldsPtr)lds;
   Tile t;
@@ -601,8 +672,20 @@ __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
   const uint32_t slabs = (t.kLen + P::kSlab - 1) / P::kSlab;
   // The slabs s + SM of the m side and s + SN of the n side, into the buffers of slab s.
   uint32_t curN = 0, curM = SN * P::kLdsN, leftN = t.kLen, leftM = t.kLen;
+  uint32_t touched = kOutside;
+  if constexpr (TOUCH) {
+    const uint32_t rn = t.m0 / BM % 8 * 32 + lane, rm = t.n0 / BN % 4 * 64 + lane;
+    if (wave == 0 && lane < 32 && rn < a.n - t.n0) touched = (uint32_t)(rn * a.ldn * P::ES);
+    if (wave == 1 && rm < t.mEnd - t.m0) touched = (uint32_t)(rm * a.ldm * P::ES);
+  }
   auto issueN = [&] {
     sn.issue(lds0 + curN, wave, leftN);
+    if constexpr (TOUCH) {                    // sn.at is a slab further already, and sm.at too
+      const uint64_t from = (wave == 0 ? sn.at : sm.at) + (kTouchAhead - 1) * 128;
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)from, 0, 0x7fffffff, 0x00020000);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds0 + kLds),
+                   "v"(leftN > kTouchAhead * P::kSlab ? touched : kOutside), "s"(rsrc));
+    }
     leftN = leftN > P::kSlab ? leftN - P::kSlab : 0;
     curN = curN + P::kLdsN < SN * P::kLdsN ? curN + P::kLdsN : 0;
   };
@@ -618,11 +701,11 @@ __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
       if (q < SM) issueM();
       issueN();
     }
-    waitAndMeet<(SM - 1) * kLoadsM + (SN - 1) * kLoadsN>();
+    waitAndMeet<(SM - 1) * kLoadsM + (SN - 1) * kLoadsN + TOUCH>();
     const char *ln = lds, *lm = lds + SN * P::kLdsN;
     auto nextSlab = [&] {
       FX_FENCE();
-      waitAndMeet<(SM - 2) * kLoadsM + (SN - 2) * kLoadsN>();
+      waitAndMeet<(SM - 2) * kLoadsM + (SN - 2) * kLoadsN + TOUCH>();
       issueM();
       issueN();
       ln = lds + curN;
@@ -936,10 +1019,10 @@ inline flagcxResult_t launchGrid(const void *kernel, ProductArgs &a, uint32_t bn
 }
 
 // SN = 0: guarded
-template <class T, class Out, int BN, int BM, int WN, int WM, int SN, int SM, bool NACROSS, bool MACROSS, bool DW>
+template <class T, class Out, int BN, int BM, int WN, int WM, int SN, int SM, bool NACROSS, bool MACROSS, bool DW, bool TOUCH = false>
 flagcxResult_t launchTiles(ProductArgs a, hipStream_t s) {
   const void *kernel;
-  if constexpr (SN != 0) kernel = reinterpret_cast<const void *>(productDirect<T, Out, BN, BM, WN, WM, SN, SM, NACROSS, MACROSS, DW>);
+  if constexpr (SN != 0) kernel = reinterpret_cast<const void *>(productDirect<T, Out, BN, BM, WN, WM, SN, SM, NACROSS, MACROSS, DW, TOUCH>);
   else kernel = reinterpret_cast<const void *>(productGuarded<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
   return launchGrid(kernel, a, BN, BM, DW, WN * WM * 64, s);
 }
@@ -1020,6 +1103,8 @@ flagcxResult_t launchShapes(const ProductArgs &a, hipStream_t s) {
   constexpr bool kLargest = !__is_same(T, E4m3Exact);
   switch (cheapestTile(a, DW, es == 1 ? kCost8 : kCost16, kLargest ? kTile256 : kTile128)) {
     case kTile256:
+      if constexpr (__is_same(T, E4m3))
+        if (a.rows / a.experts >= 2048) return launchTiles<T, Out, 256, 256, 4, 2, 2, 2, NACROSS, MACROSS, DW, true>(a, s);
       if constexpr (kLargest) return launchTiles<T, Out, 256, 256, 4, 2, kBytes<T> == 1 ? 2 : 3, 2, NACROSS, MACROSS, DW>(a, s);
     case kTile128: return launchTiles<T, Out, 128, 128, 2, 2, 2, 2, NACROSS, MACROSS, DW>(a, s);
     case kTile256x64: return launchTiles<T, Out, 256, 64, 4, 1, 3, 3, NACROSS, MACROSS, DW>(a, s);
