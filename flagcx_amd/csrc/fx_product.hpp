@@ -636,13 +636,17 @@ constexpr uint32_t kTouchAhead = 4;
 // allows.)  Loads past the last slab have no lanes inside the buffer and read nothing.
 //
 // 16 bits: two halves of the reduction, each with two groups of m fragments.
-// e4m3: a phase is one m fragment (registers: 128 of accumulators, 32 of n
+// e4m3, eight m fragments to a wavefront: a phase is one m fragment (registers: 128 of accumulators, 32 of n
 // fragments); a product of 128 goes to registers of its own and is scaled into the
 // accumulators two products later, in the shadow of the matrix instructions.
 #define FX_FENCE() __builtin_amdgcn_sched_barrier(0)
 
+// Two wavefronts to a SIMD, from one workgroup or from two, where LDS holds them.
+template <class T, int THREADS, int LDS>
+constexpr int kToSimd = THREADS >= 512 || (THREADS == 256 && 2 * LDS <= 160 * 1024 && !__is_same(T, E4m3Exact)) ? 2 : 1;
+
 template <class T, class Out, int BN, int BM, int WN, int WM, int SN, int SM, bool NACROSS, bool MACROSS, bool DW, bool TOUCH>
-__global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
+__global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * BN + SM * BM) * 128 + SM * WN * WM * 256>)) productDirect(ProductArgs a) {
   using P = Product<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>;
   constexpr uint32_t kStageM = P::kLdsM + (P::kScaled ? P::kThreads * 4 : 0), kLds = SN * P::kLdsN + SM * kStageM;
   constexpr int kLoadsN = P::N::kLoads + TOUCH, kLoadsM = P::M::kLoads + P::kScaled;   // per thread and slab
@@ -713,8 +717,62 @@ __global__ void __launch_bounds__(WN *WM * 64) productDirect(ProductArgs a) {
     };
     if (t.m0 + p.wm >= t.mEnd) {              // an expert's last tile: no row for this wavefront
       for (uint32_t s = 0; s < slabs; s++) nextSlab();
-    } else
-    if constexpr (P::kScaled) {
+    } else if constexpr (P::kScaled && P::FM <= 4) {
+      // Small e4m3 tiles: all of a slab's fragments are read a slab ahead.
+      struct Slab {
+        u32x4 n[P::FN][2], m[P::FM][2];
+        float scale[P::FM];
+      } even, odd;
+      float blocks = 0.f;                     // lane l: the block's scale of slab 64 * (s / 64) + l
+      auto read = [&](Slab &b) {
+#pragma unroll
+        for (int f = 0; f < P::FN; f++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) b.n[f][h] = p.readN(ln, f, h);
+#pragma unroll
+        for (int q = 0; q < P::FM; q++) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) b.m[q][h] = p.readM(lm, q, h);
+          b.scale[q] = *reinterpret_cast<const float *>(lm + P::kLdsM + (p.wm + p.i * P::FM + q) * 4);
+        }
+      };
+      auto multiply = [&](const Slab &b, uint32_t s) {
+        if ((s & 63) == 0) blocks = s + lane < slabs ? blockScale[s + lane] : 0.f;
+        const float sb = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, blocks), (int)(s & 63)));
+        f32x4 part[3];
+        float w[P::FM];
+        auto scaled = [&](int at) {
+          const int f = at % P::FN, q = at / P::FN;
+#pragma unroll
+          for (int v = 0; v < 4; v++) p.acc[f][q][v] = __builtin_fmaf(part[at % 3][v], w[q], p.acc[f][q][v]);
+          asm volatile("" : "+v"(p.acc[f][q]));   // see below
+        };
+#pragma unroll
+        for (int q = 0; q < P::FM; q++) w[q] = b.scale[q] * sb;
+#pragma unroll
+        for (int at = 0; at < P::FM * P::FN; at++) {
+          part[at % 3] = mma8<T>(b.n[at % P::FN], b.m[at / P::FN]);
+          if (at >= 2) scaled(at - 2);
+          FX_FENCE();
+        }
+        scaled(P::FM * P::FN - 2);
+        scaled(P::FM * P::FN - 1);
+      };
+      auto step = [&](uint32_t s, const Slab &now, Slab &then) {
+        nextSlab();
+        FX_FENCE();
+        read(then);
+        FX_FENCE();
+        multiply(now, s);
+      };
+      read(even);
+      uint32_t s = 0;
+      for (; s + 1 < slabs; s += 2) {
+        step(s, even, odd);
+        step(s + 1, odd, even);
+      }
+      if (s < slabs) step(s, even, odd);
+    } else if constexpr (P::kScaled) {
       u32x4 n[P::FN][2], m[2][2];
       f32x4 part[3];
       float scale[2];
