@@ -1098,34 +1098,42 @@ inline bool wholeChunks(const void *p, size_t ld, size_t expert, size_t inner, s
 }
 
 // The tiles of the direct kernels: extent, workgroups that a compute unit holds,
-// and what one slab takes a workgroup, in tenths of a microsecond: alone on its
-// compute unit (`alone`, from calls with fewer workgroups than units: 32 .. 256 rows,
-// n = k = 8192) and with all units full (`full`, from 8192^3).  Large tiles multiply
-// faster, small ones fill the chip with less; the fastest by this account is taken.
+// what one slab takes a workgroup, in tenths of a microsecond: alone on its
+// compute unit (`alone`, from calls with fewer workgroups than units: 64 .. 256 rows,
+// n = k = 8192) and with all units full (`full`, from 8192^3), and the rate at which
+// weights arrive (`rate`, TB/s, from 8 rows each of 32 experts, 4096 x 4096).  Large
+// tiles multiply and read faster, small ones fill the chip with less; a smaller tile
+// is taken where this account puts it a fifth ahead (it does not know that smaller
+// tiles read their operands more often: 128 rows each of 32 experts take 228 us in
+// tiles of 256 and 278 us in tiles of 128, where the account says 207 and 184).
 struct TileCost {
   uint32_t bn, bm, held;
-  float alone, full;
+  float alone, full, rate;
 };
 enum { kTile256, kTile128, kTile256x64, kTile128x64, kTile64, kTiles };
-constexpr TileCost kCost16[kTiles] = {{256, 256, 1, 13.3f, 16.2f}, {128, 128, 2, 8.2f, 4.8f}, {256, 64, 1, 7.2f, 6.2f},
-                                      {128, 64, 2, 4.5f, 2.95f}, {64, 64, 2, 3.4f, 1.94f}};
-constexpr TileCost kCost8[kTiles] = {{256, 256, 1, 20.f, 20.5f}, {128, 128, 2, 11.7f, 6.6f}, {256, 64, 1, 13.2f, 11.4f},
-                                     {128, 64, 2, 9.5f, 4.0f}, {64, 64, 2, 8.6f, 3.1f}};
+constexpr TileCost kCost16[kTiles] = {{256, 256, 1, 13.3f, 16.2f, 6.1f}, {128, 128, 2, 8.2f, 4.7f, 5.9f}, {256, 64, 1, 7.2f, 6.2f, 5.9f},
+                                      {128, 64, 2, 4.6f, 2.9f, 5.1f}, {64, 64, 2, 3.4f, 1.9f, 4.3f}};
+constexpr TileCost kCost8[kTiles] = {{256, 256, 1, 20.f, 20.5f, 6.1f}, {128, 128, 2, 10.1f, 5.8f, 5.9f}, {256, 64, 1, 11.6f, 9.8f, 5.9f},
+                                     {128, 64, 2, 8.1f, 3.7f, 5.1f}, {64, 64, 2, 7.4f, 3.0f, 4.3f}};
 
-inline int cheapestTile(const ProductArgs &a, bool dw, const TileCost *cost, int first) {
+inline int cheapestTile(const ProductArgs &a, bool dw, size_t es, const TileCost *cost, int first) {
+  const float reached = (float)(a.experts < a.rows ? a.experts : a.rows);
+  const float slabs = dw ? (float)a.rows / a.experts / 64 : (float)a.k * es / 128;
+  const float bytes = dw ? 0.f : reached * a.n * a.k * es;
   int best = first;
   float least = 0.f;
   for (int c = first; c < kTiles; c++) {
     // an expert's last tile is half full on average, and takes half the time
     const float m = dw ? (float)((a.m + cost[c].bm - 1) / cost[c].bm) * a.experts
-                       : (a.offsets ? (float)a.rows / cost[c].bm + 0.5f * (a.experts < a.rows ? a.experts : a.rows)
-                                    : (float)((a.rows + cost[c].bm - 1) / cost[c].bm));
+                       : (a.offsets ? (float)a.rows / cost[c].bm + 0.5f * reached : (float)((a.rows + cost[c].bm - 1) / cost[c].bm));
     const float tiles = m * (float)((a.n + cost[c].bn - 1) / cost[c].bn);
     const uint32_t slots = kUnits * cost[c].held, rounds = (uint32_t)(tiles / slots);
     const float rest = tiles - (float)rounds * slots;
     const float deep = (float)(uint32_t)((rest + kUnits - 1) / kUnits) * cost[c].full;   // workgroups sharing a unit in the last round
-    const float t = rounds * cost[c].held * cost[c].full + (rest > 0 ? (deep > cost[c].alone ? deep : cost[c].alone) : 0.f);
-    if (c == first || t < least) {
+    const float multiply = slabs * 0.1f * (rounds * cost[c].held * cost[c].full + (rest > 0 ? (deep > cost[c].alone ? deep : cost[c].alone) : 0.f));
+    const float read = bytes / (cost[c].rate * 1e6f);
+    const float t = multiply > read ? multiply : read;
+    if (c == first || t < 0.8f * least) {
       least = t;
       best = c;
     }
@@ -1159,7 +1167,7 @@ flagcxResult_t launchShapes(const ProductArgs &a, hipStream_t s) {
   if (!direct) return launchTiles<T, Out, 128, 128, 2, 2, 0, 0, NACROSS, MACROSS, DW>(a, s);
   // widened e4m3 operands leave no registers for the largest tile
   constexpr bool kLargest = !__is_same(T, E4m3Exact);
-  switch (cheapestTile(a, DW, es == 1 ? kCost8 : kCost16, kLargest ? kTile256 : kTile128)) {
+  switch (cheapestTile(a, DW, es, es == 1 ? kCost8 : kCost16, kLargest ? kTile256 : kTile128)) {
     case kTile256:
       if constexpr (__is_same(T, E4m3))
         if (a.rows / a.experts >= 2048) return launchTiles<T, Out, 256, 256, 4, 2, 2, 2, NACROSS, MACROSS, DW, true>(a, s);
