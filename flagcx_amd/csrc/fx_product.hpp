@@ -187,12 +187,12 @@ __device__ __forceinline__ bool findTileDw(const ProductArgs &a, Tile *t) {
 // ------------------------------------------------------- one operand's tile
 
 // Chunk exchange of an "along" tile.  On the m side the sixteen lanes of a
-// fragment are rows 16 f + i; on the n side rows 16 (i / 4) + 4 f + i % 4 of a
-// block of 64, which gives a lane sixteen consecutive columns over its four
-// fragments.
+// fragment are rows 16 f + i; on the n side rows 8 (i / 4) + i % 4, + 4 in odd
+// fragments, of a block of 32, which gives a lane eight consecutive columns over two
+// fragments and the four lane groups a row's 32.
 template <bool NSIDE>
 __device__ __forceinline__ uint32_t exchange(uint32_t r) {
-  return NSIDE ? ((r & 3) | ((r >> 2) & 4)) : (r & 7);
+  return NSIDE ? ((r & 3) | ((r >> 1) & 4)) : (r & 7);
 }
 
 // R = extent of the tile in its own index, NT = threads, ES = bytes per element.
@@ -204,11 +204,7 @@ struct Side {
   static constexpr int kElems = 16 / ES;
   static constexpr uint32_t kSlab = 128 / ES;            // reduction elements per slab
 
-  // A thread's chunks lie in rows that the exchange treats alike, except where its
-  // rows are 16 apart on the n side.
-  static constexpr bool kTurns = NSIDE && !ACROSS && kStep % 32 != 0;
-  static_assert(ACROSS ? kStep % 4 == 0 : kStep % 16 == 0, "rows that the exchange treats alike");
-  __device__ __forceinline__ uint32_t element(int q) const { return (chunk ^ (kTurns && (q & 1) ? 4u : 0u)) * kElems; }
+  static_assert(kStep % (ACROSS ? 4 : 16) == 0, "a thread's chunks lie in rows that the exchange treats alike");
 
   // position of this thread's first chunk
   uint32_t row, chunk;
@@ -222,7 +218,7 @@ struct Side {
   // index 0 at reduction 0.  own / red: how much of the tile's own index and of the
   // slab's reduction exists.
   __device__ __forceinline__ u32x4 guarded(const char *base, size_t ld, int i, uint32_t own, uint32_t red) const {
-    const uint32_t r = row + i * kStep, c = element(i);
+    const uint32_t r = row + i * kStep, c = chunk * kElems;
     u32x4 v = {};
     const uint32_t rows = ACROSS ? red : own, cols = ACROSS ? own : red;
     if (r >= rows || c >= cols) return v;
@@ -244,7 +240,7 @@ struct Side {
 // Fragment reads.  lane l: index i = l % 16 of the fragment, reduction group g = l / 16.
 template <bool NSIDE>
 __device__ __forceinline__ u32x4 readAlong(const char *lds, uint32_t wave0, int f, int half, uint32_t i, uint32_t g) {
-  const uint32_t r = NSIDE ? wave0 + (f >> 2) * 64 + 16 * (i >> 2) + 4 * (f & 3) + (i & 3) : wave0 + 16 * f + i;
+  const uint32_t r = NSIDE ? wave0 + 32 * (f >> 1) + 8 * (i >> 2) + 4 * (f & 1) + (i & 3) : wave0 + 16 * f + i;
   return *reinterpret_cast<const u32x4 *>(lds + r * 128 + (((uint32_t)(half * 4) + g) ^ exchange<NSIDE>(r)) * 16);
 }
 template <int R>
@@ -325,63 +321,45 @@ __device__ __forceinline__ void storeRun(Out *p, uint32_t c, uint32_t cols, cons
   }
 }
 
-// Four fragments side by side, of each of which a lane of group g holds columns
-// 4 g .. 4 g + 3: turned over the four groups, so that group g holds all sixteen
-// columns of fragment g and a row's 64 leave in pieces of 32 bytes or more.
-__device__ __forceinline__ void turn4(uint32_t (&w)[4]) {
-  auto swap16 = [](uint32_t &x, uint32_t &y) {   // odd groups of x against even groups of y
-    const auto r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
-    x = r[0];
-    y = r[1];
-  };
-  auto swap32 = [](uint32_t &x, uint32_t &y) {   // groups 2, 3 of x against 0, 1 of y
-    const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
-    x = r[0];
-    y = r[1];
-  };
-  swap16(w[0], w[1]);
-  swap16(w[2], w[3]);
-  swap32(w[0], w[2]);
-  swap32(w[1], w[3]);
-  // now w[0], w[1], w[2], w[3]: the first, second, third and last four columns
+// Two fragments side by side, of each of which a lane of group g holds columns
+// 4 g .. 4 g + 3: exchanged between the lane groups so that group g holds columns
+// 8 g .. 8 g + 7 of the 32, the first four in x and the others in y, and a store
+// writes a row's columns without gaps.
+__device__ __forceinline__ void sideBySide(uint32_t &x, uint32_t &y) {
+  const auto halves = __builtin_amdgcn_permlane32_swap(x, y, false, false);            // groups 2, 3 of x against 0, 1 of y
+  const auto quarters = __builtin_amdgcn_permlane16_swap(halves[0], halves[1], false, false);   // 1, 3 against 0, 2
+  x = quarters[0];
+  y = quarters[1];
 }
 template <class Out>
-__device__ __forceinline__ void storeTurned(Out *row, uint32_t c, uint32_t cols, const f32x4 (&part)[4]) {
-  float v[16];
+__device__ __forceinline__ void storeAcross(Out *row, uint32_t c, uint32_t cols, f32x4 a, f32x4 b) {
   if constexpr (sizeof(Out) == 4) {
+    float v[8];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      uint32_t w[4];
-#pragma unroll
-      for (int f = 0; f < 4; f++) {
-        const float x = part[f][j];           // a value: __builtin_bit_cast of a vector's element takes the first
-        w[f] = __builtin_bit_cast(uint32_t, x);
-      }
-      turn4(w);
-#pragma unroll
-      for (int h = 0; h < 4; h++) v[4 * h + j] = __builtin_bit_cast(float, w[h]);
+      const float fa = a[j], fb = b[j];       // values: __builtin_bit_cast of a vector's element takes the first
+      uint32_t x = __builtin_bit_cast(uint32_t, fa), y = __builtin_bit_cast(uint32_t, fb);
+      sideBySide(x, y);
+      v[j] = __builtin_bit_cast(float, x);
+      v[4 + j] = __builtin_bit_cast(float, y);
     }
     storeRun(row, c, cols, v);
   } else {
-    uint32_t out[8];
+    u32x4 w;
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      uint32_t w[4];
-#pragma unroll
-      for (int f = 0; f < 4; f++)
-        w[f] = (uint32_t)__builtin_bit_cast(uint16_t, (Out)part[f][2 * j]) |
-               ((uint32_t)__builtin_bit_cast(uint16_t, (Out)part[f][2 * j + 1]) << 16);
-      turn4(w);
-#pragma unroll
-      for (int h = 0; h < 4; h++) out[2 * h + j] = w[h];
+      uint32_t x = (uint32_t)__builtin_bit_cast(uint16_t, (Out)a[2 * j]) | ((uint32_t)__builtin_bit_cast(uint16_t, (Out)a[2 * j + 1]) << 16);
+      uint32_t y = (uint32_t)__builtin_bit_cast(uint16_t, (Out)b[2 * j]) | ((uint32_t)__builtin_bit_cast(uint16_t, (Out)b[2 * j + 1]) << 16);
+      sideBySide(x, y);
+      w[j] = x;
+      w[2 + j] = y;
     }
-    if (c + 16 <= cols) {
-      *reinterpret_cast<u32x4_anywhere *>(row + c) = u32x4{out[0], out[1], out[2], out[3]};
-      *reinterpret_cast<u32x4_anywhere *>(row + c + 8) = u32x4{out[4], out[5], out[6], out[7]};
+    if (c + 8 <= cols) {
+      *reinterpret_cast<u32x4_anywhere *>(row + c) = w;
     } else {
 #pragma unroll
-      for (int j = 0; j < 16; j++)
-        if (c + j < cols) reinterpret_cast<uint16_t *>(row)[c + j] = (uint16_t)(out[j >> 1] >> (16 * (j & 1)));
+      for (int j = 0; j < 8; j++)
+        if (c + j < cols) reinterpret_cast<uint16_t *>(row)[c + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
     }
   }
 }
@@ -466,19 +444,16 @@ struct Product {
       const bool live = m < t.mEnd;
       if (!NACROSS && !live) continue;        // the across form exchanges between lanes first
       Out *row = y + (size_t)m * a.ldy;
-      if constexpr (NACROSS) {
 #pragma unroll
-        for (int b = 0; b < FN / 4; b++) {
-          const f32x4 part[4] = {acc[4 * b][q], acc[4 * b + 1][q], acc[4 * b + 2][q], acc[4 * b + 3][q]};
-          storeTurned<Out>(row, live ? t.n0 + wn + 64 * b + 16 * g : a.n, a.n, part);
-        }
-      } else {
+      for (int b = 0; b < FN / 2; b++) {
+        const uint32_t c = t.n0 + wn + 32 * b + 8 * g;
+        if constexpr (NACROSS) {
+          storeAcross<Out>(row, live ? c : a.n, a.n, acc[2 * b][q], acc[2 * b + 1][q]);
+        } else {
+          float v[8];
 #pragma unroll
-        for (int b = 0; b < FN / 4; b++) {
-          float v[16];
-#pragma unroll
-          for (int j = 0; j < 16; j++) v[j] = acc[4 * b + (j >> 2)][q][j & 3];
-          storeRun(row, t.n0 + wn + 64 * b + 16 * g, a.n, v);
+          for (int j = 0; j < 8; j++) v[j] = acc[2 * b + (j >> 2)][q][j & 3];
+          storeRun(row, c, a.n, v);
         }
       }
     }
@@ -584,14 +559,14 @@ struct DirectSide : Side<R, NT, ES, ACROSS, NSIDE> {
     advance = ACROSS ? S::kSlab * ld * ES : 128;
 #pragma unroll
     for (int q = 0; q < S::kLoads; q++)
-      voff[q] = (ACROSS ? S::element(q) < own : S::row + q * S::kStep < own) ? (uint32_t)((S::row * ld + S::element(q)) * ES) : kOutside;
+      voff[q] = (ACROSS ? S::chunk * S::kElems < own : S::row + q * S::kStep < own) ? (uint32_t)((S::row * ld + S::chunk * S::kElems) * ES) : kOutside;
   }
   // red: reduction elements left from this slab on
   __device__ __forceinline__ void issue(uint32_t lds, uint32_t wave, uint32_t red) {
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)at, 0, 0x7fffffff, 0x00020000);
 #pragma unroll
     for (int q = 0; q < S::kLoads; q++) {
-      const bool there = ACROSS ? S::row + q * S::kStep < red : S::element(q) < red;
+      const bool there = ACROSS ? S::row + q * S::kStep < red : S::chunk * S::kElems < red;
       loadToLds(lds + (q * NT + wave * 64) * 16, there ? voff[q] : kOutside, rsrc, q * step);
     }
     at += advance;
