@@ -87,6 +87,7 @@ __device__ __forceinline__ uint32_t rowsOf(const ProductArgs &a, uint32_t e, uin
 // neighbours: a die's L2 then holds the operands of a block of kPanel row tiles by
 // a few column tiles.
 constexpr uint32_t kDies = 8, kPanel = 8, kGroup = 4, kUnits = 256;
+constexpr int kKinds = 5;   // whole tiles, and last tiles by quarters
 __device__ __forceinline__ uint32_t dieOrder(uint32_t id, uint32_t total) {
   const uint32_t die = id % kDies, at = id / kDies, q = total / kDies, r = total % kDies;
   return die * q + (die < r ? die : r) + at;
@@ -101,9 +102,9 @@ __device__ __forceinline__ void panelOrder(uint32_t id, uint32_t mTiles, uint32_
 // The row tiles of all experts are counted on the device (the host knows only an
 // upper bound, the grid): every wavefront scans the boundaries, 64 experts at a time.
 // ORDERED: kGroup columns of tiles at a time, first the whole tiles of all experts,
-// then the experts' last tiles with more than half their rows, then the others, which
-// take half the time and fill up the end of the call.  A group's weights are used by
-// both while the memory-side cache holds them.
+// then the experts' last tiles, by the quarter of their rows that they have: they
+// take that much less time, and the shortest fill up the end of the call.  A group's
+// weights are used by whole and last tiles while the memory-side cache holds them.
 template <int BN, int BM, bool ORDERED>
 __device__ __forceinline__ bool findTile(const ProductArgs &a, Tile *t) {
   uint32_t mt, nt, id = blockIdx.x;
@@ -115,25 +116,34 @@ __device__ __forceinline__ bool findTile(const ProductArgs &a, Tile *t) {
     return true;
   }
   const uint32_t lane = threadIdx.x & 63;
-  uint32_t first = 0, rows = 0, scan = 0, tiles[3] = {0, 0, 0};
-  // Tiles of kind 0 of this lane's expert; kinds 1 and 2 are one at most.
+  uint32_t first = 0, rows = 0, scan = 0, tiles[kKinds] = {};
+  // Tiles of kind 0 of this lane's expert; of the others it has one at most.
   auto whole = [&] { return ORDERED ? rows / BM : (rows + BM - 1) / BM; };
-  auto isKind = [&](int k) { return ORDERED && rows % BM != 0 && (rows % BM > BM / 2) == (k == 1); };
+  auto isKind = [&](int k) { return ORDERED && rows % BM != 0 && (int)((rows % BM - 1) / (BM / 4)) == 4 - k; };
   for (uint32_t e = 0; e < a.experts; e += 64) {
     rows = rowsOf(a, e + lane, &first);
     scan = waveScan(whole());
     tiles[0] += uniform((uint32_t)__shfl((int)scan, 63));
-    tiles[1] += (uint32_t)__popcll(__ballot(isKind(1)));
-    tiles[2] += (uint32_t)__popcll(__ballot(isKind(2)));
+#pragma unroll
+    for (int k = 1; k < kKinds; k++) tiles[k] += (uint32_t)__popcll(__ballot(isKind(k)));
   }
-  const uint32_t mTiles = tiles[0] + tiles[1] + tiles[2];
+  uint32_t mTiles = 0;
+#pragma unroll
+  for (int k = 0; k < kKinds; k++) mTiles += tiles[k];
   if (id >= mTiles * a.nTiles) return false;
   const uint32_t wide = ORDERED ? kGroup : a.nTiles, group = id / (mTiles * wide);
   const uint32_t left = a.nTiles - group * wide, w = left < wide ? left : wide;   // columns of tiles in this group
   id -= group * mTiles * wide;
   int kind = 0;
-  while (kind < 2 && id >= tiles[kind] * w) id -= tiles[kind++] * w;
-  const uint32_t at = dieOrder(id, tiles[kind] * w);
+  uint32_t all = tiles[0];
+#pragma unroll
+  for (int k = 1; k < kKinds; k++)
+    if (kind == k - 1 && id >= all * w) {
+      id -= all * w;
+      kind = k;
+      all = tiles[k];
+    }
+  const uint32_t at = dieOrder(id, all * w);
   mt = at / w;
   nt = group * wide + at % w;
   for (uint32_t e = 0, before = 0; e < a.experts; e += 64) {
@@ -690,7 +700,10 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
       ln = lds + curN;
       lm = lds + curM;
     };
-    if (t.m0 + p.wm >= t.mEnd) {              // an expert's last tile: no row for this wavefront
+    // An expert's last tile may have no row for this wavefront, or rows for half of its
+    // fragments at most.
+    const bool few = !DW && t.m0 + p.wm + P::TM / 2 >= t.mEnd;
+    if (t.m0 + p.wm >= t.mEnd) {
       for (uint32_t s = 0; s < slabs; s++) nextSlab();
     } else if constexpr (P::kScaled && P::FM <= 4) {
       // Small e4m3 tiles: all of a slab's fragments are read a slab ahead.
@@ -752,48 +765,53 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
       f32x4 part[3];
       float scale[2];
       float blocks = 0.f;                     // lane l: the block's scale of slab 64 * (s / 64) + l
-      auto readM = [&](int q) {
-        const int fragment = q % P::FM;
-        m[q & 1][0] = p.readM(lm, fragment, 0);
-        m[q & 1][1] = p.readM(lm, fragment, 1);
-        scale[q & 1] = *reinterpret_cast<const float *>(lm + P::kLdsM + (p.wm + p.i * P::FM + fragment) * 4);
+      auto readM = [&](int buffer, int fragment) {
+        m[buffer][0] = p.readM(lm, fragment, 0);
+        m[buffer][1] = p.readM(lm, fragment, 1);
+        scale[buffer] = *reinterpret_cast<const float *>(lm + P::kLdsM + (p.wm + p.i * P::FM + fragment) * 4);
       };
       auto readN = [&](int f) {
         n[f][0] = p.readN(ln, f, 0);
         n[f][1] = p.readN(ln, f, 1);
       };
-      readM(0);
+      auto walk = [&](auto fragments) {
+        constexpr int Q = decltype(fragments)::value;
+        static_assert(Q % 2 == 0, "fragment 0 goes to buffer 0");
+        readM(0, 0);
 #pragma unroll
-      for (int f = 0; f < P::FN; f++) readN(f);
-      for (uint32_t s = 0; s < slabs; s++) {
-        if ((s & 63) == 0) blocks = s + lane < slabs ? blockScale[s + lane] : 0.f;
-        const float sb = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, blocks), (int)(s & 63)));
-        float w[P::FM];
-        auto scaled = [&](int at) {           // product `at` into its accumulators
-          const int f = at % P::FN, q = at / P::FN;
+        for (int f = 0; f < P::FN; f++) readN(f);
+        for (uint32_t s = 0; s < slabs; s++) {
+          if ((s & 63) == 0) blocks = s + lane < slabs ? blockScale[s + lane] : 0.f;
+          const float sb = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, blocks), (int)(s & 63)));
+          float w[Q];
+          auto scaled = [&](int at) {           // product `at` into its accumulators
+            const int f = at % P::FN, q = at / P::FN;
 #pragma unroll
-          for (int v = 0; v < 4; v++) p.acc[f][q][v] = __builtin_fmaf(part[at % 3][v], w[q], p.acc[f][q][v]);
-          asm volatile("" : "+v"(p.acc[f][q]));   // here, not sunk behind the slab with all products alive
-        };
+            for (int v = 0; v < 4; v++) p.acc[f][q][v] = __builtin_fmaf(part[at % 3][v], w[q], p.acc[f][q][v]);
+            asm volatile("" : "+v"(p.acc[f][q]));   // here, not sunk behind the slab with all products alive
+          };
 #pragma unroll
-        for (int q = 0; q < P::FM; q++) {
-          if (q == P::FM - 1) nextSlab();
-          FX_FENCE();
-          w[q] = scale[q & 1] * sb;
-          readM(q + 1);                       // FM is even: FM is fragment 0 of the next slab, in buffer 0
-          FX_FENCE();
-#pragma unroll
-          for (int f = 0; f < P::FN; f++) {
-            const int at = q * P::FN + f;
-            part[at % 3] = mma8<T>(n[f], m[q & 1]);
-            if (at >= 2) scaled(at - 2);
+          for (int q = 0; q < Q; q++) {
+            if (q == Q - 1) nextSlab();
             FX_FENCE();
-            if (q == P::FM - 1) readN(f);
+            w[q] = scale[q & 1] * sb;
+            readM((q + 1) & 1, (q + 1) % Q);
+            FX_FENCE();
+#pragma unroll
+            for (int f = 0; f < P::FN; f++) {
+              const int at = q * P::FN + f;
+              part[at % 3] = mma8<T>(n[f], m[q & 1]);
+              if (at >= 2) scaled(at - 2);
+              FX_FENCE();
+              if (q == Q - 1) readN(f);
+            }
           }
+          scaled(Q * P::FN - 2);
+          scaled(Q * P::FN - 1);
         }
-        scaled(P::FM * P::FN - 2);
-        scaled(P::FM * P::FN - 1);
-      }
+      };
+      if (few) walk(std::integral_constant<int, P::FM / 2>());
+      else walk(std::integral_constant<int, P::FM>());
     } else {
       constexpr int GQ = P::FM / 2;
       u32x4 n[2][P::FN], m[2][GQ];
@@ -801,31 +819,36 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
 #pragma unroll
         for (int f = 0; f < P::FN; f++) n[half][f] = p.readN(ln, f, half);
       };
-      auto readM = [&](int ph) {
+      auto walk = [&](auto groups) {            // of m fragments
+        constexpr int G = decltype(groups)::value, kPhases = 2 * G;
+        auto readM = [&](int ph) {
 #pragma unroll
-        for (int j = 0; j < GQ; j++) m[ph & 1][j] = p.readM(lm, (ph & 1) * GQ + j, ph >> 1);
-      };
-      readN(0);
-      readM(0);
-      for (uint32_t s = 0; s < slabs; s++) {
+          for (int j = 0; j < GQ; j++) m[ph & 1][j] = p.readM(lm, ph % G * GQ + j, ph / G);
+        };
+        readN(0);
+        readM(0);
+        for (uint32_t s = 0; s < slabs; s++) {
 #pragma unroll
-        for (int ph = 0; ph < 4; ph++) {
-          if (ph == 3) nextSlab();
-          FX_FENCE();
-          readM((ph + 1) & 3);
-          if (ph == 0) readN(1);
-          if (ph == 3) readN(0);
-          FX_FENCE();
+          for (int ph = 0; ph < kPhases; ph++) {
+            if (ph == kPhases - 1) nextSlab();
+            FX_FENCE();
+            readM((ph + 1) % kPhases);
+            if (ph == 0) readN(1);
+            if (ph == kPhases - 1) readN(0);
+            FX_FENCE();
 #pragma unroll
-          for (int j = 0; j < GQ; j++)
+            for (int j = 0; j < GQ; j++)
 #pragma unroll
-            for (int f = 0; f < P::FN; f++) {
-              const int q = (ph & 1) * GQ + j;
-              p.acc[f][q] = mma<T>(n[ph >> 1][f], m[ph & 1][j], p.acc[f][q]);
-            }
-          FX_FENCE();
+              for (int f = 0; f < P::FN; f++) {
+                const int q = ph % G * GQ + j;
+                p.acc[f][q] = mma<T>(n[ph / G][f], m[ph & 1][j], p.acc[f][q]);
+              }
+            FX_FENCE();
+          }
         }
-      }
+      };
+      if (few) walk(std::integral_constant<int, 1>());
+      else walk(std::integral_constant<int, 2>());
     }
   }
   // The loads behind the last slab have to have ended before this workgroup's LDS is another's.
