@@ -26,7 +26,7 @@ struct NormArgs {
   float *scale;
   const void *weight;
   size_t ldIn, ldRes, ldTotal, ldOut, ldScale;
-  uint32_t rows, cols, n;                     // n = entries of `in`
+  uint32_t row0, rows, cols, n;               // rows [row0, rows) of this launch; n = entries of `in`
   uint32_t k;
   float eps;
   uint32_t weightF32;
@@ -129,7 +129,7 @@ template <class T, int V, bool WAVE, bool QUANT, bool STREAM>
 __global__ void __launch_bounds__(WAVE ? 256 : 1024) normRows(NormArgs a) {
   __shared__ float lds[16];
   const uint32_t threads = WAVE ? 64 : blockDim.x, t = WAVE ? threadIdx.x & 63 : threadIdx.x;
-  const uint32_t row = WAVE ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const uint32_t row = a.row0 + (WAVE ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x);
   if (row >= a.rows) return;                  // whole wavefronts leave, and there is no barrier then
   uint32_t c[V];
 #pragma unroll
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(WAVE ? 256 : 1024) normRows(NormArgs a) {
 template <class T, bool QUANT>
 __global__ void __launch_bounds__(1024) normLongRows(NormArgs a) {
   __shared__ float lds[16];
-  const uint32_t row = blockIdx.x;
+  const uint32_t row = a.row0 + blockIdx.x;
   const uint32_t steps = (a.cols + 1024 * 8 - 1) / (1024 * 8);
   float q = 0.f;
   for (uint32_t s = 0; s < steps; s++) {
@@ -182,7 +182,7 @@ struct NormGradArgs {
   uint32_t ldPartial;                         // columns rounded up to 32
   float *rms;                                 // long rows: 1 / rms per row for the column kernel
   size_t ldDy, ldX, ldDtotal, ldDx;
-  uint32_t rows, cols;
+  uint32_t row0, rows, cols;                  // row0: long rows
   float eps;
   uint32_t weightF32;
 };
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(THREADS) normGradRows(NormGradArgs a) {
 template <class T>
 __global__ void __launch_bounds__(1024) normGradLongRows(NormGradArgs a) {
   __shared__ float lds[16];
-  const uint32_t row = blockIdx.x;
+  const uint32_t row = a.row0 + blockIdx.x;
   const uint32_t steps = (a.cols + 1024 * 8 - 1) / (1024 * 8);
   float q = 0.f, m = 0.f;
   for (uint32_t s = 0; s < steps; s++) {
@@ -430,20 +430,35 @@ constexpr size_t kMaxExtent = 0x7fffffe0;   // also when rounded up to 32
 constexpr uint32_t kFewRows = 512;
 constexpr uint64_t kStreamBytes = 32u << 20, kGradStreamBytes = 128u << 20;
 
+// One launch for every kRowsAtATime rows, `per` of them to a workgroup: the runtime
+// takes at most 2^32 threads.
+constexpr uint32_t kRowsAtATime = 1u << 22;
+template <class K, class A>
+flagcxResult_t launchByRow(K kernel, A a, uint32_t per, uint32_t threads, hipStream_t s) {
+  const uint32_t rows = a.rows;
+  flagcxResult_t rc = flagcxSuccess;
+  for (uint32_t r = 0; r < rows && rc == flagcxSuccess; r += kRowsAtATime) {
+    a.row0 = r;
+    a.rows = rows - r < kRowsAtATime ? rows : r + kRowsAtATime;
+    rc = launchShape(kernel, dim3((a.rows - r + per - 1) / per), threads, s, a);
+  }
+  return rc;
+}
+
 // Wavefronts that hold `octets`, v to a lane, in threads.
 uint32_t threadsFor(uint32_t octets, uint32_t v) { return ((octets + v - 1) / v + 63) / 64 * 64; }
 
 template <class T, bool QUANT, bool STREAM>
 flagcxResult_t launchNormRows(const NormArgs &a, hipStream_t s) {
-  const uint32_t octets = (a.cols + 7) / 8, fours = (a.rows + 3) / 4;
-  if (octets <= 64) return launchShape(normRows<T, 1, true, QUANT, STREAM>, dim3(fours), 256, s, a);
+  const uint32_t octets = (a.cols + 7) / 8;
+  if (octets <= 64) return launchByRow(normRows<T, 1, true, QUANT, STREAM>, a, 4, 256, s);
   // Few rows: one octet to a lane, so that all inputs of a row are on their way at once (one row of 8192 with eight
   // inputs 8.4 -> 6.4 us).
   if constexpr (!STREAM)
-    if (octets <= 1024 && a.rows <= kFewRows) return launchShape(normRows<T, 1, false, QUANT, STREAM>, dim3(a.rows), threadsFor(octets, 1), s, a);
-  if (octets <= 128) return launchShape(normRows<T, 2, true, QUANT, STREAM>, dim3(fours), 256, s, a);
-  if (octets <= 512) return launchShape(normRows<T, 2, false, QUANT, STREAM>, dim3(a.rows), threadsFor(octets, 2), s, a);
-  return launchShape(normRows<T, 4, false, QUANT, STREAM>, dim3(a.rows), threadsFor(octets, 4), s, a);
+    if (octets <= 1024 && a.rows <= kFewRows) return launchByRow(normRows<T, 1, false, QUANT, STREAM>, a, 1, threadsFor(octets, 1), s);
+  if (octets <= 128) return launchByRow(normRows<T, 2, true, QUANT, STREAM>, a, 4, 256, s);
+  if (octets <= (sizeof(T) == 4 ? 2048 : 512)) return launchByRow(normRows<T, 2, false, QUANT, STREAM>, a, 1, threadsFor(octets, 2), s);
+  return launchByRow(normRows<T, 4, false, QUANT, STREAM>, a, 1, threadsFor(octets, 4), s);
 }
 
 // Results that the dies' L2s (32 MiB) cannot hold are streamed (16384 x 8192, two bf16
@@ -453,7 +468,7 @@ flagcxResult_t launchNormRows(const NormArgs &a, hipStream_t s) {
 // written (1024 x 4096).
 template <class T, bool QUANT>
 flagcxResult_t launchNorm(const NormArgs &a, hipStream_t s) {
-  if (a.cols > kHeld) return launchShape(normLongRows<T, QUANT>, dim3(a.rows), 1024, s, a);
+  if (a.cols > kHeld) return launchByRow(normLongRows<T, QUANT>, a, 1, 1024, s);
   const uint64_t written = (uint64_t)a.rows * a.cols * ((a.total ? sizeof(T) : 0) + (QUANT ? 1 : sizeof(T)));
   return written > kStreamBytes ? launchNormRows<T, QUANT, true>(a, s) : launchNormRows<T, QUANT, false>(a, s);
 }
@@ -501,12 +516,12 @@ flagcxResult_t launchGrad(NormGradArgs a, void *dweight, bool weightF32, void *w
       a.rms = (float *)workspace + (size_t)parts * a.ldPartial;
       NormGradArgs b = a;
       b.dx = nullptr;
-      rc = launchShape(normGradLongRows<T>, dim3(a.rows), 1024, s, b);
+      rc = launchByRow(normGradLongRows<T>, b, 1, 1024, s);
       if (rc != flagcxSuccess) return rc;
       rc = launchShape(normGradLongColumns<T>, dim3((a.cols + 2047) / 2048, parts), 256, s, b);
       if (rc != flagcxSuccess) return rc;
     }
-    if (a.dx) rc = launchShape(normGradLongRows<T>, dim3(a.rows), 1024, s, a);
+    if (a.dx) rc = launchByRow(normGradLongRows<T>, a, 1, 1024, s);
   } else if (a.rows) {
     // What the memory-side cache cannot keep is streamed both ways (8192 x 4096 bf16: 54 -> 50 us, 8192 x 8192: 107 ->
     // 95 us).
@@ -558,6 +573,7 @@ int fx_reduce_norm(void *out, float *scale, void *total, const void *const *in, 
   a.ldTotal = st.total;
   a.ldOut = st.out;
   a.ldScale = st.scale;
+  a.row0 = 0;
   a.rows = (uint32_t)rows;
   a.cols = (uint32_t)cols;
   a.k = (uint32_t)k;
@@ -606,6 +622,7 @@ int fx_reduce_norm_grad(void *dx, void *dweight, const void *dy, const void *x, 
   a.ldX = st.x;
   a.ldDtotal = st.dtotal;
   a.ldDx = st.dx;
+  a.row0 = 0;
   a.rows = (uint32_t)rows;
   a.cols = (uint32_t)cols;
   a.eps = eps;

@@ -158,11 +158,14 @@ __device__ __forceinline__ bool findTile(const ProductArgs &a, Tile *t) {
       const uint32_t ahead = kind ? (uint32_t)__builtin_amdgcn_mbcnt_hi((uint32_t)(set >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0))
                                   : scan - whole();
       const bool mine = kind ? isKind(kind) && ahead == want : ahead <= want && want < scan;
-      const uint32_t l = (uint32_t)__builtin_ctzll(__ballot(mine));
+      const uint64_t one = __ballot(mine);
+      if (!one) return false;                        // boundaries that changed between two readings
+      const uint32_t l = (uint32_t)__builtin_ctzll(one);
       const uint32_t skip = kind ? rows / BM : want - ahead;                // tiles of the same expert in front
       const uint32_t f = uniform((uint32_t)__shfl((int)first, (int)l)), r = uniform((uint32_t)__shfl((int)rows, (int)l));
-      *t = Tile{e + l, f + uniform((uint32_t)__shfl((int)skip, (int)l)) * BM, f + r, nt * BN, 0, a.k};
-      return true;
+      const uint32_t m0 = f + uniform((uint32_t)__shfl((int)skip, (int)l)) * BM;
+      *t = Tile{e + l, m0, f + r, nt * BN, 0, a.k};
+      return m0 < f + r;
     }
     before += here;
   }
@@ -185,7 +188,8 @@ __device__ __forceinline__ bool findTileDw(const ProductArgs &a, Tile *t) {
         const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)rows, (int)j);
         rank += other > rows || (other == rows && j < lane);
       }
-      e = (uint32_t)__builtin_ctzll(__ballot(lane < a.experts && rank == turn));
+      const uint64_t one = __ballot(lane < a.experts && rank == turn);
+      e = one ? (uint32_t)__builtin_ctzll(one) : turn;
     }
     rows = uniform(rowsOf(a, e, &first));
     first = uniform(first);
@@ -1069,7 +1073,7 @@ inline flagcxResult_t launchGrid(const void *kernel, ProductArgs &a, uint32_t bn
   else if (!a.offsets) a.mTiles = (a.rows + bm - 1) / bm;
   else a.mTiles = a.rows / bm + (a.experts < a.rows ? a.experts : a.rows);   // every expert's last tile may be partial
   const uint64_t grid = (uint64_t)a.nTiles * a.mTiles * (dw ? a.experts : 1);
-  if (grid > 0x7fffffffu) return flagcxNotSupported;
+  if (grid * threads > 0xffffffffu) return flagcxNotSupported;   // the runtime's limit: 2^32 threads
   void *argv[] = {&a};
   return hipLaunchKernel(kernel, dim3((uint32_t)grid), dim3(threads), argv, 0, s) == hipSuccess ? flagcxSuccess : flagcxUnhandledDeviceError;
 }
@@ -1161,7 +1165,7 @@ flagcxResult_t launchShapes(const ProductArgs &a, hipStream_t s) {
     if (near && each <= most) return launchThin<T, Out, 2, 4, 4, 1>(a, s);
   }
   const bool direct = wholeChunks(a.pn, a.ldn, a.expertN, NACROSS ? a.n : a.k, es) &&
-                      wholeChunks(a.pm, a.ldm, 0, MACROSS ? a.m : a.k, es);
+                      wholeChunks(a.pm, a.ldm, 0, MACROSS ? a.m : a.k, es) && a.ldsm < (1u << 20);
   if (!direct) return launchTiles<T, Out, 128, 128, 2, 2, 0, 0, NACROSS, MACROSS, DW>(a, s);
   // widened e4m3 operands leave no registers for the largest tile
   constexpr bool kLargest = !__is_same(T, E4m3Exact);

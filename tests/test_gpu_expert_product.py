@@ -342,3 +342,120 @@ def test_products_replay_in_a_graph_with_new_routing(dev, rows, n, k):
         hip.hipGraphExecDestroy(gexec)
         hip.hipGraphDestroy(graph)
     dev.stream_destroy(stream)
+
+
+@pytest.mark.parametrize("rows", [20, 1500])
+def test_weights_and_rows_far_apart(dev, rows):
+    """Offsets beyond 32 bits: experts 2.4 GB apart, and rows so far apart that the direct loads' offsets do not reach."""
+    n, k, experts, t = 264, 136, 3, N.DT_BF16
+    far = 1_200_000_000
+    x, w = R.normal(t, (rows, k), 1), R.normal(t, (experts, n, k), 2)
+    o = np.array([0, rows // 4, rows // 2, rows], np.int32)
+    want, mag = R.product(R.codes_to_f64(x, t), R.codes_to_f64(w, t), o, True)
+    with DevBufs(dev) as b:
+        dx, do, dy = b.put(x), b.put(o), b.alloc(rows * n * 2)
+        dw = b.alloc((far * (experts - 1) + n * k) * 2)
+        for e in range(experts):
+            dev.upload(dw + 2 * far * e, np.ascontiguousarray(w[e]))
+        st = dict(x=k, w=k, y=n, expert_w=far)
+        N.check(K.expert_product(dy, dx, dw, do, experts, rows, n, k, t, strides=st))
+        dev.sync()
+        got = R.codes_to_f64(dev.to_host(dy, rows * n, np.uint16).reshape(rows, n), t)
+        assert (np.abs(got - want) <= R.rounding(want, t) * 1.01 + R.sum_bound(k, mag)).all()
+        dev.free(b.ptrs.pop())
+        ld = (5 << 30) // 2 // rows // 8 * 8                           # rows of x spread over 5 GB
+        dfar, dw2 = b.alloc(rows * ld * 2), b.put(w)
+        for r in range(rows):
+            dev.upload(dfar + r * ld * 2, np.ascontiguousarray(x[r]))
+        st = dict(x=ld, w=k, y=n, expert_w=n * k)
+        N.check(K.expert_product(dy, dfar, dw2, do, experts, rows, n, k, t, strides=st))
+        dev.sync()
+        got = R.codes_to_f64(dev.to_host(dy, rows * n, np.uint16).reshape(rows, n), t)
+        assert (np.abs(got - want) <= R.rounding(want, t) * 1.01 + R.sum_bound(k, mag)).all()
+        # the weights' gradient walks the same far rows
+        dyv = R.normal(t, (rows, n), 5)
+        ddy, ddw = b.put(dyv), b.alloc(experts * n * k * 4)
+        st = dict(dy=n, x=ld, dw=k, expert_dw=n * k)
+        N.check(K.expert_product_dw(ddw, ddy, dfar, do, experts, rows, n, k, t, out_dtype=N.DT_FP32, strides=st))
+        dev.sync()
+        gw = dev.to_host(ddw, experts * n * k, np.float32).reshape(experts, n, k).astype(np.float64)
+    want, mag = R.product_dw(R.codes_to_f64(dyv, t), R.codes_to_f64(x, t), o)
+    assert (np.abs(gw - want) <= R.rounding(want, N.DT_FP32) * 1.01 + R.sum_bound(rows, mag)).all()
+
+
+def test_products_on_two_streams_at_once(dev):
+    rows, n, k, experts, t = 900, 520, 264, 5, N.DT_BF16
+    rng = np.random.default_rng(4)
+    streams = [dev.stream_create() for _ in range(2)]
+    with DevBufs(dev) as b:
+        sets = []
+        for i in range(2):
+            sets.append((b.alloc(rows * n * 2), b.put(R.normal(t, (rows, k), i)), b.put(R.normal(t, (experts, n, k), 7 + i)),
+                         b.put(ragged(rows, experts, rng)), b.alloc(experts * n * k * 2)))
+            dev.memset(sets[-1][0], 0, rows * n * 2)
+        dev.sync()
+
+        def call(s, raw):
+            N.check(K.expert_product(s[0], s[1], s[2], s[3], experts, rows, n, k, t, stream=raw))
+            N.check(K.expert_product_dw(s[4], s[0], s[1], s[3], experts, rows, n, k, t, stream=raw))
+        read = lambda s: (dev.to_host(s[0], rows * n, np.uint16), dev.to_host(s[4], experts * n * k, np.uint16))  # noqa: E731
+        alone = []
+        for s in sets:
+            call(s, None)
+            dev.sync()
+            alone.append(read(s))
+        for _ in range(10):
+            for s, st in zip(sets, streams):
+                call(s, dev.raw_stream(st))
+        dev.sync()
+        for s, a in zip(sets, alone):
+            got = read(s)
+            assert np.array_equal(got[0], a[0]) and np.array_equal(got[1], a[1])
+    for st in streams:
+        dev.stream_destroy(st)
+
+
+@pytest.mark.parametrize("rest", [1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 191, 192, 193, 255])
+def test_last_tiles_of_every_length(dev, rest):
+    """Experts whose last tile has `rest` rows, in the smallest and the largest tile shapes."""
+    o = np.cumsum([0, 256 + rest, rest, 0, 512, rest]).astype(np.int32)
+    for n, k in ((200, 72), (4104, 128)):
+        run(dev, N.DT_BF16, int(o[-1]) + 3, n, k, o, seed=rest)
+        run(dev, N.DT_FP16, int(o[-1]) + 3, n, k, o, seed=rest, nk=False)
+        run8(dev, int(o[-1]) + 3, n // 16 * 16, k // 16 * 16, o, N.DT_BF16, seed=rest)
+
+
+@pytest.mark.parametrize("rests", [(1, 64, 130, 200), (63, 65, 129, 193), (255, 192, 128, 16)])
+def test_last_tiles_among_many_large_ones(dev, rests):
+    o = np.cumsum([0, 2048 + rests[0], 1536 + rests[1], 0, rests[2], 4096 + rests[3]]).astype(np.int32)
+    rows = int(o[-1]) + 5
+    for nk in (True, False):
+        run(dev, N.DT_BF16, rows, 4168, 136, o, nk=nk, seed=rests[0])
+    run8(dev, rows, 4176, 272, o, N.DT_BF16, seed=rests[0])
+    run8(dev, rows, 4176, 144, o, N.DT_FP32, seed=rests[0])
+
+
+def test_e4m3_long_reduction_in_large_tiles(dev):
+    """Long enough for the lines that are touched ahead, with and without a partial slab at the end."""
+    for k in (1024, 1040, 2064):
+        run8(dev, 3200, 4160, k, None, N.DT_BF16, seed=k)
+        run8(dev, 4500, 4160, k, np.array([0, 2100, 4400], np.int32), N.DT_BF16, seed=k)
+
+
+def test_infinities_and_nan_stay_in_their_rows(dev):
+    """A row with a NaN or an infinity spoils its own results alone, also where its tile's other rows belong to another
+    expert; a weight with one spoils its own column."""
+    for rows, n, k in ((40, 136, 264), (700, 264, 136)):
+        x, w = R.normal(N.DT_BF16, (rows, k), 1), R.normal(N.DT_BF16, (2, n, k), 2)
+        x[rows // 2, 3], x[rows // 2 + 1, k - 1] = 0x7fc0, 0x7f80
+        w[1, 7, k - 1] = 0x7fc0
+        o = np.array([0, rows // 2 + 1, rows], np.int32)
+        with DevBufs(dev) as b:
+            dx, dw, do, dy = b.put(x), b.put(w), b.put(o), b.alloc(rows * n * 4)
+            N.check(K.expert_product(dy, dx, dw, do, 2, rows, n, k, N.DT_BF16, out_dtype=N.DT_FP32))
+            dev.sync()
+            y = dev.to_host(dy, rows * n, np.float32).reshape(rows, n)
+        assert np.isnan(y[rows // 2]).all() and not np.isfinite(y[rows // 2 + 1]).any()
+        assert np.isnan(y[rows // 2 + 1:, 7]).all()
+        rest = np.delete(y, [rows // 2, rows // 2 + 1], axis=0)
+        assert np.isfinite(rest[:rows // 2]).all() and np.isfinite(np.delete(rest, 7, axis=1)).all()

@@ -278,3 +278,58 @@ def test_norm_and_gradients_replay_in_a_graph(dev):
         hip.hipGraphExecDestroy(gexec)
         hip.hipGraphDestroy(graph)
     dev.stream_destroy(stream)
+
+
+def test_norm_rows_far_apart_and_many(dev):
+    """Offsets beyond 32 bits: rows 16 MiB apart (4.8 GB from first to last), and more rows than one launch takes."""
+    rows, cols, ld = 300, 640, 8 << 20
+    x = R.normal(N.DT_BF16, (rows, cols), 3)
+    with DevBufs(dev) as b:
+        dx, dt = b.alloc(rows * ld * 2), b.alloc(rows * ld * 2)
+        for r in (0, 1, 150, rows - 1):
+            dev.upload(dx + r * ld * 2, np.ascontiguousarray(x[r]))
+        st = dict(in_=ld, residual=ld, total=ld, out=ld, scale=5)
+        N.check(K.reduce_norm(dt, [dx], None, rows, cols, N.DT_BF16, eps=EPS, strides=st))
+        dev.sync()
+        for r in (0, 1, 150, rows - 1):
+            f = R.codes_to_f64(x[r:r + 1], N.DT_BF16)
+            s, y, mag, q = R.norm([f], None, None, EPS)
+            got = R.codes_to_f64(dev.to_host(dt + r * ld * 2, cols, np.uint16), N.DT_BF16)
+            assert (np.abs(got - y[0]) <= R.rounding(y[0], N.DT_BF16) * 1.01 + R.norm_bounds(s, y, mag, q, None, 1)[1][0]).all(), r
+    rows, cols = (1 << 22) + 1003, 8
+    x = R.normal(N.DT_BF16, (rows, cols), 4)
+    with DevBufs(dev) as b:
+        dx, dt = b.put(x), b.alloc(rows * cols * 2)
+        N.check(K.reduce_norm(dt, [dx], None, rows, cols, N.DT_BF16, eps=EPS))
+        dev.sync()
+        got = R.codes_to_f64(dev.to_host(dt, rows * cols, np.uint16).reshape(rows, cols)[-3000:], N.DT_BF16)
+    s, y, mag, q = R.norm([R.codes_to_f64(x[-3000:], N.DT_BF16)], None, None, EPS)
+    assert (np.abs(got - y) <= R.rounding(y, N.DT_BF16) * 1.01 + R.norm_bounds(s, y, mag, q, None, 1)[1]).all()
+
+
+def test_norm_gradients_on_two_streams_with_a_workspace_each(dev):
+    rows, cols, t = 700, 2000, N.DT_BF16
+    need = K.reduce_norm_grad_workspace(rows, cols)
+    streams = [dev.stream_create() for _ in range(2)]
+    with DevBufs(dev) as b:
+        sets = []
+        for i in range(2):
+            x, dy, w = R.normal(t, (rows, cols), 10 + i), R.normal(t, (rows, cols), 20 + i), R.normal(t, (cols,), 30 + i)
+            sets.append((b.put(x), b.put(dy), b.put(w), b.alloc(rows * cols * 2), b.alloc(cols * 2), b.alloc(need)))
+        dev.sync()
+        call = lambda s, raw: N.check(K.reduce_norm_grad(s[3], s[4], s[1], s[0], s[2], rows, cols, t, s[5], need, eps=EPS, stream=raw))  # noqa: E731
+        read = lambda s: (dev.to_host(s[3], rows * cols, np.uint16), dev.to_host(s[4], cols, np.uint16))  # noqa: E731
+        alone = []
+        for s in sets:
+            call(s, None)
+            dev.sync()
+            alone.append(read(s))
+        for _ in range(10):
+            for s, st in zip(sets, streams):
+                call(s, dev.raw_stream(st))
+        dev.sync()
+        for s, a in zip(sets, alone):
+            got = read(s)
+            assert np.array_equal(got[0], a[0]) and np.array_equal(got[1], a[1])
+    for st in streams:
+        dev.stream_destroy(st)
