@@ -1112,10 +1112,10 @@ struct TileCost {
   uint32_t bn, bm, held;
   float alone, full, rate;
 };
-enum { kTile256, kTile128, kTile256x64, kTile128x64, kTile64, kTiles };
-constexpr TileCost kCost16[kTiles] = {{256, 256, 1, 13.3f, 16.2f, 6.1f}, {128, 128, 2, 8.2f, 4.7f, 5.9f}, {256, 64, 1, 7.2f, 6.2f, 5.9f},
+enum { kTile256, kTile128, kTile128x64, kTile64, kTiles };
+constexpr TileCost kCost16[kTiles] = {{256, 256, 1, 13.3f, 16.2f, 6.1f}, {128, 128, 2, 8.2f, 4.7f, 5.9f},
                                       {128, 64, 2, 4.6f, 2.9f, 5.1f}, {64, 64, 2, 3.4f, 1.9f, 4.3f}};
-constexpr TileCost kCost8[kTiles] = {{256, 256, 1, 20.f, 20.5f, 6.1f}, {128, 128, 2, 10.1f, 5.8f, 5.9f}, {256, 64, 1, 11.6f, 9.8f, 5.9f},
+constexpr TileCost kCost8[kTiles] = {{256, 256, 1, 20.f, 20.5f, 6.1f}, {128, 128, 2, 10.1f, 5.8f, 5.9f},
                                      {128, 64, 2, 8.1f, 3.7f, 5.1f}, {64, 64, 2, 7.4f, 3.0f, 4.3f}};
 
 inline int cheapestTile(const ProductArgs &a, bool dw, size_t es, const TileCost *cost, int first) {
@@ -1175,7 +1175,6 @@ flagcxResult_t launchShapes(const ProductArgs &a, hipStream_t s) {
         if (a.rows / a.experts >= 2048) return launchTiles<T, Out, 256, 256, 4, 2, 2, 2, NACROSS, MACROSS, DW, true>(a, s);
       if constexpr (kLargest) return launchTiles<T, Out, 256, 256, 4, 2, kBytes<T> == 1 ? 2 : 3, 2, NACROSS, MACROSS, DW>(a, s);
     case kTile128: return launchTiles<T, Out, 128, 128, 2, 2, 2, 2, NACROSS, MACROSS, DW>(a, s);
-    case kTile256x64: return launchTiles<T, Out, 256, 64, 4, 1, 3, 3, NACROSS, MACROSS, DW>(a, s);
     case kTile128x64: return launchTiles<T, Out, 128, 64, 2, 2, 3, 3, NACROSS, MACROSS, DW>(a, s);
     default: return launchTiles<T, Out, 64, 64, 1, 2, 4, 4, NACROSS, MACROSS, DW>(a, s);
   }

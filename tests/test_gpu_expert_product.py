@@ -88,7 +88,9 @@ def test_ragged_products(dev, nk, rows, experts, n, k):
 def test_sizes_between_few_rows_and_full_tiles(dev, nk, rows, experts, n, k):
     """Where the tile's shape depends on how many tiles there are."""
     rng = np.random.default_rng(n)
-    run(dev, N.DT_BF16, rows, n, k, None if experts == 1 else ragged(rows, experts, rng), nk=nk, seed=k)
+    for t in (N.DT_BF16, N.DT_FP16):
+        for out32 in (False, True):
+            run(dev, t, rows, n, k, None if experts == 1 else ragged(rows, experts, rng), nk=nk, out32=out32, seed=k)
 
 
 @pytest.mark.parametrize("nk", [True, False])
@@ -197,6 +199,39 @@ def test_large_weight_gradients(dev):
         run_dw(dev, N.DT_FP16, rows, n, k, None if experts == 1 else ragged(rows, experts, rng), pad=pad, seed=k, out32=pad == 8)
 
 
+@pytest.mark.parametrize("experts", [1, 2, 4, 8])
+def test_weight_gradients_of_middling_sizes(dev, experts):
+    rng = np.random.default_rng(experts)
+    for t in (N.DT_BF16, N.DT_FP16):
+        for out32 in (False, True):
+            run_dw(dev, t, 300, 1032, 1032, ragged(300, experts, rng), out32=out32, seed=experts)
+
+
+def test_few_rows_of_many_columns(dev):
+    """A workgroup for every 32 columns fills the chip: one expert's rows, and a row each of many experts."""
+    rng = np.random.default_rng(1)
+    for rows, experts, n, k in ((1, 1, 8200, 136), (16, 1, 8200, 1000), (13, 1, 8201, 65), (40, 40, 520, 264), (100, 64, 264, 72)):
+        o = None if experts == 1 else ragged(rows, experts, rng)
+        print(rows, experts, n, k, flush=True)
+        for t in (N.DT_BF16, N.DT_FP16):
+            run(dev, t, rows, n, k, o, seed=k, out32=t == N.DT_FP16)
+        for out in (N.DT_BF16, N.DT_FP16, N.DT_FP32):
+            run8(dev, rows, n, k, o, out, seed=k)
+    for rows, n, k in ((28, 1000, 520), (60, 1000, 520)):
+        run(dev, N.DT_BF16, rows, n, k, None, seed=k, out32=True)
+        run8(dev, rows, n, k, None, N.DT_BF16, seed=k)
+
+
+def test_large_products_in_32_bits(dev):
+    for nk in (True, False):
+        run(dev, N.DT_BF16, 3200, 4160, 200, None, nk=nk, out32=True, seed=1)
+        run(dev, N.DT_FP16, 3300, 4168, 136, None, nk=nk, out32=True, seed=2, pad=8)
+        run(dev, N.DT_FP16, 3300, 4168, 136, None, nk=nk, seed=3)
+    for t in (N.DT_BF16, N.DT_FP16):
+        for out32 in (False, True):
+            run(dev, t, 200, 263, 135, None, out32=out32, seed=4)      # nothing aligned
+
+
 def test_weight_gradient_without_rows_is_zero(dev):
     with DevBufs(dev) as b:
         dw, o = b.put(np.full((2, 5, 7), 3, np.uint16)), b.put(np.zeros(3, np.int32))
@@ -272,7 +307,7 @@ def test_e4m3_ragged_products(dev, rows, experts, n, k):
                                               (1000, 20, 1296, 272), (1900, 32, 2064, 144), (4000, 30, 1040, 272)])
 def test_e4m3_sizes_between_few_rows_and_full_tiles(dev, rows, experts, n, k):
     rng = np.random.default_rng(n)
-    for out in (N.DT_BF16, N.DT_FP32):
+    for out in (N.DT_BF16, N.DT_FP16, N.DT_FP32):
         run8(dev, rows, n, k, None if experts == 1 else ragged(rows, experts, rng), out, seed=k)
 
 
