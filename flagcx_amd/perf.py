@@ -7,11 +7,13 @@ algBw = bytes / 1e9 / t).  Usage:
     python -m flagcx_amd.perf pack              # alltoallv pack / unpack
     python -m flagcx_amd.perf allreduce -n 8 -d bf16 -b 1M -e 64M [--graph]
     python -m flagcx_amd.perf fifo -b 4K -e 256M -f 8   # round trips through the reduce FIFO
+    python -m flagcx_amd.perf norm -k 2 -d bf16 --cols 8192 -b 1 -e 16K -f 8   # k-way sum + residual + norm over rows, its gradients
+    python -m flagcx_amd.perf experts -d bf16 --experts 16 --cols 4096 --width 4096 -b 16 -e 16K -f 4   # products grouped by expert
     python -m flagcx_amd.perf coldstart         # library sizes and the first call's latency (code-object load)
 
 Warm and cold.  Every figure is "warm" unless --cold is given: the same buffers
 are used launch after launch, so whatever of them fits MI355X's 256 MiB
-memory-side cache is served from it.  With --cold (reduce, slices, pack) every
+memory-side cache is served from it.  With --cold (reduce, slices, pack, norm) every
 timed launch is preceded by a 1 GiB fill with ordinary stores that pushes the
 operands out of that cache, and is timed by its own pair of events; both
 columns are printed.  reduce --fresh adds the case a reduction meets when it
@@ -233,6 +235,73 @@ def run_pack(dev, a):
     row("pack, 8 x 4,194,304 el aligned", sum(big) * 4, t.both(lambda: N.check(K.pack(dpk, dbig, big, bd, N.DT_FP32, t.raw)), a.cold), 2 * sum(big) * 4)
     row("pack, 8 x 4,194,304 el, source off by 1 el", sum(big) * 4,
         t.ms(lambda: N.check(K.pack(dpk, dbig + 4, big, bd, N.DT_FP32, t.raw))), 2 * sum(big) * 4)
+
+
+def _normal(dev, n, dtype, seed):
+    p = dev.malloc(max(n, 1) * N.DTYPE_SIZE[dtype] + 64)
+    dev.upload(p, K.synth(max(n, 1), dtype, K.SYNTH_NORMAL, 0.0, 1.0, seed))
+    return p
+
+
+def run_norm(dev, a):
+    """What a tensor-parallel layer does with the ranks' partial results: the sum of k
+    inputs and the residual, normed to the inputs' type and to e4m3 with scales, and
+    the gradients, for -b .. -e rows of --cols columns."""
+    t = Timer(dev)
+    dtype, k, c = DT[a.dtype], a.k, a.cols
+    es, rmax = N.DTYPE_SIZE[dtype], size(a.max)
+    ins = [_normal(dev, rmax * c, dtype, p) for p in range(k)]
+    res, w = _normal(dev, rmax * c, dtype, 90), _normal(dev, c, dtype, 91)
+    tot, out, scale = (dev.malloc(rmax * c * es) for _ in range(3))
+    space = K.reduce_norm_grad_workspace(rmax, c)
+    ws, dw = dev.malloc(space + 64), dev.malloc(c * es)
+    r = size(a.min)
+    while r <= rmax:
+        n = r * c * es
+        call = lambda **kw: N.check(K.reduce_norm(out, ins, w, r, c, dtype, eps=1e-6, residual=res, total=tot, stream=t.raw, **kw))  # noqa: B023,E731
+        row(f"norm {r} x {c} k={k} {a.dtype}", n, t.both(call, a.cold), n * (k + 3))
+        row(f"norm {r} x {c} k={k} {a.dtype} to e4m3", n,
+            t.both(lambda: call(scale=scale, out_dtype=N.DT_E4M3), a.cold), n * (k + 2) + r * c + 4 * r * -(-c // 128))
+        row(f"norm gradients {r} x {c} {a.dtype}", n, t.both(lambda: N.check(K.reduce_norm_grad(  # noqa: B023
+            out, dw, res, ins[0], w, r, c, dtype, ws, space, eps=1e-6, dtotal=tot, stream=t.raw)), a.cold), 4 * n)
+        r *= a.factor
+
+
+def run_experts(dev, a):
+    """Products grouped by expert: -b .. -e rows of --cols columns, dealt to --experts
+    experts unevenly, each with weights of --width x --cols; both gradients, and the
+    e4m3 form."""
+    t = Timer(dev)
+    dtype = DT[a.dtype]
+    e, k, n, rmax = a.experts, a.cols, a.width, size(a.max)
+    x, w, dy = _normal(dev, rmax * k, dtype, 1), _normal(dev, e * n * k, dtype, 2), _normal(dev, rmax * n, dtype, 3)
+    y, dx, dw = dev.malloc(rmax * n * 2), dev.malloc(rmax * k * 2), dev.malloc(e * n * k * 2)
+    kg, ng = -(-k // 128), -(-n // 128)
+    xs, ws = (dev.to_device(np.full(m, 2.0 ** -8, np.float32)) for m in (rmax * kg, e * ng * kg))
+    x8, w8 = (dev.to_device(np.random.default_rng(i).integers(0x28, 0x50, m, dtype=np.uint8)) for i, m in enumerate((rmax * k, e * n * k)))
+    off, rows = dev.malloc(4 * (e + 1)), size(a.min)
+
+    def line(what, fn, nbytes, flops):
+        ms = t.ms(fn)
+        print(f"{what:<52s} {ms * 1e3:10.2f} us   {flops / ms / 1e9:8.1f} TFLOP/s   {nbytes / ms / 1e6:8.1f} GB/s", flush=True)
+
+    while rows <= rmax:
+        share = np.random.default_rng(rows).dirichlet(np.full(e, 4.0))
+        o = np.concatenate([[0], np.floor(np.cumsum(share) * rows + 0.5)]).astype(np.int32)
+        o[-1] = rows
+        dev.upload(off, o)
+        reached = int((np.diff(o) > 0).sum())
+        fl, by = 2.0 * rows * n * k, 2 * (reached * n * k + rows * (n + k))
+        name = f"{rows} rows, {e} experts {n} x {k}"
+        line(f"y = x W^T   {name} {a.dtype}", lambda: N.check(K.expert_product(y, x, w, off, e, rows, n, k, dtype, stream=t.raw)), by, fl)
+        line(f"dx = dy W   {name} {a.dtype}",
+             lambda: N.check(K.expert_product(dx, dy, w, off, e, rows, k, n, dtype, layout=K.W_KN, stream=t.raw)), by, fl)
+        line(f"dW = dy^T x {name} {a.dtype}", lambda: N.check(K.expert_product_dw(dw, dy, x, off, e, rows, n, k, dtype, stream=t.raw)),
+             2 * (e * n * k + rows * (n + k)), fl)
+        line(f"y = x W^T   {name} e4m3",
+             lambda: N.check(K.expert_product_e4m3(y, x8, xs, w8, ws, off, e, rows, n, k, N.DT_BF16, stream=t.raw)),
+             reached * n * k + rows * (2 * n + k), fl)
+        rows *= a.factor
 
 
 def run_fifo(dev, a):
@@ -511,7 +580,8 @@ def run_coldstart():
 
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("what", choices=["reduce", "slices", "pack", "allreduce", "fifo", "collectives", "torchref", "coldstart"])
+    ap.add_argument("what", choices=["reduce", "slices", "pack", "allreduce", "fifo", "collectives", "norm", "experts", "torchref",
+                                         "coldstart"])
     ap.add_argument("--cold", action="store_true",
                     help="reduce / slices / pack: also time every launch after a 1 GiB fill that empties the caches")
     ap.add_argument("--fresh", action="store_true",
@@ -536,6 +606,9 @@ def main(argv=None):
                     help="reduce: place the k inputs and the output in ONE allocation, STRIDE bytes apart (e.g. 512M, 16G)")
     ap.add_argument("--in-shift", type=int, default=0,
                     help="start input i at byte offset i*IN_SHIFT of its allocation (multiple of 16 keeps vector loads)")
+    ap.add_argument("--cols", type=int, default=4096, help="norm: columns of a row; experts: length of the reduction")
+    ap.add_argument("--width", type=int, default=4096, help="experts: columns of the result")
+    ap.add_argument("--experts", type=int, default=16)
     a = ap.parse_args(argv)
     if a.what == "torchref":         # torch brings its own HIP runtime: nothing of this library is loaded beside it
         return run_torchref()
@@ -543,7 +616,7 @@ def main(argv=None):
         return run_coldstart()
     dev = Device(0)
     {"reduce": run_reduce, "slices": run_slices, "pack": run_pack, "allreduce": run_allreduce,
-     "fifo": run_fifo, "collectives": run_collectives}[a.what](dev, a)
+     "fifo": run_fifo, "collectives": run_collectives, "norm": run_norm, "experts": run_experts}[a.what](dev, a)
 
 
 if __name__ == "__main__":

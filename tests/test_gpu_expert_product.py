@@ -214,7 +214,8 @@ def test_few_rows_of_many_columns(dev):
         o = None if experts == 1 else ragged(rows, experts, rng)
         print(rows, experts, n, k, flush=True)
         for t in (N.DT_BF16, N.DT_FP16):
-            run(dev, t, rows, n, k, o, seed=k, out32=t == N.DT_FP16)
+            for out32 in (False, True):
+                run(dev, t, rows, n, k, o, seed=k, out32=out32)
         for out in (N.DT_BF16, N.DT_FP16, N.DT_FP32):
             run8(dev, rows, n, k, o, out, seed=k)
     for rows, n, k in ((28, 1000, 520), (60, 1000, 520)):
