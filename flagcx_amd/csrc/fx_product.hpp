@@ -575,6 +575,7 @@ struct DirectSide : Side<R, NT, ES, ACROSS, NSIDE> {
     for (int q = 0; q < S::kLoads; q++)
       voff[q] = (ACROSS ? S::chunk * S::kElems < own : S::row + q * S::kStep < own) ? (uint32_t)((S::row * ld + S::chunk * S::kElems) * ES) : kOutside;
   }
+  __device__ __forceinline__ void skip(int64_t slabs) { at += slabs * (int64_t)advance; }
   // red: reduction elements left from this slab on
   __device__ __forceinline__ void issue(uint32_t lds, uint32_t wave, uint32_t red) {
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)at, 0, 0x7fffffff, 0x00020000);
@@ -615,6 +616,7 @@ struct DirectScales {
 // order; the wait for a slab leaves the last touch out, so it has two slabs' time.
 // (8192^3 from memory 633 -> 579 us; where few tiles share weights it gains nothing.)
 constexpr uint32_t kTouchAhead = 4;
+constexpr uint32_t kTurn = 37;
 
 // The slabs as a pipeline.  A slab is multiplied in phases; the fragments of
 // the next phase are read from LDS while this one's are multiplied.  In front of
@@ -664,7 +666,30 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
   }
   const uint32_t slabs = (t.kLen + P::kSlab - 1) / P::kSlab;
   // The slabs s + SM of the m side and s + SN of the n side, into the buffers of slab s.
-  uint32_t curN = 0, curM = SN * P::kLdsN, leftN = t.kLen, leftM = t.kLen;
+  // left: reduction elements from the next slab to the end, 0 when all have been issued.
+  // Experts start their walk at different slabs and wrap around: rows lie a power of two
+  // apart more often than not, and all workgroups at the same slab meet on the same
+  // memory channels, while an expert's own workgroups share what they read (64 rows each
+  // of 16 experts, 4096 x 4096: 130 -> 99 us; 16 each of 64 experts: 249 -> 176 us).
+  const uint32_t turn = DW || !slabs ? 0 : t.expert * kTurn % slabs;
+  uint32_t curN = 0, curM = SN * P::kLdsN, leftN = t.kLen - turn * P::kSlab, leftM = leftN, todoN = slabs, todoM = slabs;
+  if constexpr (!DW) {
+    sn.skip(turn);
+    sm.skip(turn);
+  }
+  if constexpr (P::kScaled) ss.at += turn * 4;
+  auto nextOf = [&](auto &side, uint32_t &left, uint32_t &todo) {
+    if constexpr (DW) {
+      left = left > P::kSlab ? left - P::kSlab : 0;
+      return false;
+    } else {
+      const bool wrap = left <= P::kSlab;
+      todo -= todo != 0;
+      if (wrap) side.skip(-(int64_t)slabs);
+      left = todo == 0 ? 0 : wrap ? t.kLen : left - P::kSlab;
+      return wrap;
+    }
+  };
   uint32_t touched = kOutside;
   if constexpr (TOUCH) {
     const uint32_t rn = t.m0 / BM % 8 * 32 + lane, rm = t.n0 / BN % 4 * 64 + lane;
@@ -679,14 +704,23 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds0 + kLds),
                    "v"(leftN > kTouchAhead * P::kSlab ? touched : kOutside), "s"(rsrc));
     }
-    leftN = leftN > P::kSlab ? leftN - P::kSlab : 0;
+    nextOf(sn, leftN, todoN);
     curN = curN + P::kLdsN < SN * P::kLdsN ? curN + P::kLdsN : 0;
   };
   auto issueM = [&] {
     sm.issue(lds0 + curM, wave, leftM);
     if constexpr (P::kScaled) ss.issue(lds0 + curM + P::kLdsM, wave, leftM != 0);
-    leftM = leftM > P::kSlab ? leftM - P::kSlab : 0;
+    const bool wrapped = nextOf(sm, leftM, todoM);
+    if constexpr (P::kScaled)
+      if (wrapped) ss.at -= (uint64_t)slabs * 4;
     curM = curM + kStageM < kLds ? curM + kStageM : SN * P::kLdsN;
+  };
+  // The block's scale of the walk's s-th slab; lane l of `blocks` holds slab 64 * (slab / 64) + l's.
+  auto scaleOf = [&](float &blocks, uint32_t s) {
+    uint32_t at = s + turn;
+    at = at < slabs ? at : at - slabs;
+    if (s == 0 || (at & 63) == 0) blocks = (at & ~63u) + lane < slabs ? blockScale[(at & ~63u) + lane] : 0.f;
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, blocks), (int)(at & 63)));
   };
   if (slabs) {
 #pragma unroll
@@ -715,7 +749,7 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
         u32x4 n[P::FN][2], m[P::FM][2];
         float scale[P::FM];
       } even, odd;
-      float blocks = 0.f;                     // lane l: the block's scale of slab 64 * (s / 64) + l
+      float blocks = 0.f;
       auto read = [&](Slab &b) {
 #pragma unroll
         for (int f = 0; f < P::FN; f++)
@@ -729,8 +763,7 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
         }
       };
       auto multiply = [&](const Slab &b, uint32_t s) {
-        if ((s & 63) == 0) blocks = s + lane < slabs ? blockScale[s + lane] : 0.f;
-        const float sb = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, blocks), (int)(s & 63)));
+        const float sb = scaleOf(blocks, s);
         f32x4 part[3];
         float w[P::FM];
         auto scaled = [&](int at) {
@@ -768,7 +801,7 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
       u32x4 n[P::FN][2], m[2][2];
       f32x4 part[3];
       float scale[2];
-      float blocks = 0.f;                     // lane l: the block's scale of slab 64 * (s / 64) + l
+      float blocks = 0.f;
       auto readM = [&](int buffer, int fragment) {
         m[buffer][0] = p.readM(lm, fragment, 0);
         m[buffer][1] = p.readM(lm, fragment, 1);
@@ -785,8 +818,7 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
 #pragma unroll
         for (int f = 0; f < P::FN; f++) readN(f);
         for (uint32_t s = 0; s < slabs; s++) {
-          if ((s & 63) == 0) blocks = s + lane < slabs ? blockScale[s + lane] : 0.f;
-          const float sb = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, blocks), (int)(s & 63)));
+          const float sb = scaleOf(blocks, s);
           float w[Q];
           auto scaled = [&](int at) {           // product `at` into its accumulators
             const int f = at % P::FN, q = at / P::FN;
@@ -1147,22 +1179,25 @@ template <class T, class Out, bool NACROSS, bool MACROSS, bool DW>
 flagcxResult_t launchShapes(const ProductArgs &a, hipStream_t s) {
   const size_t es = kBytes<T>;
   if constexpr (!NACROSS && !DW) {
-    // Few rows.  (a) up to 8 an expert: 16 at a time, 32 columns a workgroup, or 16
-    // where that leaves units without one (one row, n = k = 4096: 12.2 -> 8.3 us);
-    // eight wavefronts share the reduction, for e4m3 four (16 rows, 8192 x 8192: 19.1
-    // -> 17.0 us; bf16 31.3 -> 28.5 us the other way).  (b) up to 32 rows of one
-    // expert, 64 in e4m3 (35 us against 55 with tiles), or 12 an expert (8 rows each of
-    // 32 experts, 4096 x 4096: 202 us against 262 with tiles; 32 each: 338 against 265).
+    // Few rows.  (a) up to 8 an expert, 16 of a single one: 16 at a time, 32 columns a
+    // workgroup, or 16 where that leaves units without one (one row, n = k = 4096: 12.2 ->
+    // 8.3 us); eight wavefronts share the reduction, for e4m3 four (16 rows, 8192 x 8192:
+    // 19.1 -> 17.0 us; bf16 31.3 -> 28.5 us the other way).  (b) up to 32 rows of one
+    // expert, 64 in e4m3 (35 us against 48 with tiles).  Of several experts up to 4 rows
+    // each, or 12 where tiles of 128 columns would not fill the chip (8 each of 16 experts,
+    // 1024 x 4096: 24 us against 40; 8 each of 32, 4096 x 4096: 191 against 180).
     // The lanes' offsets have 31 bits.
     const bool near = a.ldn * es < (1u << 24) && a.ldm * es < (1u << 24) && a.ldsm < (1u << 22) &&
                       a.ldsn * (a.n / FX_SCALE_GROUP + 1) < (1u << 28) && (uint64_t)a.k * es < (1u << 30);
-    const uint64_t each = a.rows / a.experts, most = a.experts == 1 ? (es == 1 ? 64 : 32) : 12;
-    const uint64_t m = a.offsets ? a.rows / 16 + (a.experts < a.rows ? a.experts : a.rows) : (a.rows + 15) / 16;
+    const uint64_t reached = a.experts < a.rows ? a.experts : a.rows, each = a.rows / a.experts;
+    const uint64_t most = a.experts == 1 ? (es == 1 ? 64 : 32) : reached * ((a.n + 127) / 128) < 2 * kUnits ? 12 : 4;
+    const uint64_t m = a.offsets ? a.rows / 16 + reached : (a.rows + 15) / 16;
     const bool wide = m * ((a.n + 31) / 32) >= kUnits;
     constexpr int NW = kBytes<T> == 1 ? 4 : 8;
-    if (near && each <= 8) return wide ? launchThin<T, Out, 2, 1, NW, 2>(a, s) : launchThin<T, Out, 1, 1, NW, 2>(a, s);
-    if (near && each <= 16 && a.experts == 1) return wide ? launchThin<T, Out, 2, 1, NW, 2>(a, s) : launchThin<T, Out, 1, 1, NW, 2>(a, s);
-    if (near && each <= most) return launchThin<T, Out, 2, 4, 4, 1>(a, s);
+    if (near && each <= most) {
+      if (each > (a.experts == 1 ? 16 : 8)) return launchThin<T, Out, 2, 4, 4, 1>(a, s);
+      return wide ? launchThin<T, Out, 2, 1, NW, 2>(a, s) : launchThin<T, Out, 1, 1, NW, 2>(a, s);
+    }
   }
   const bool direct = wholeChunks(a.pn, a.ldn, a.expertN, NACROSS ? a.n : a.k, es) &&
                       wholeChunks(a.pm, a.ldm, 0, MACROSS ? a.m : a.k, es) && a.ldsm < (1u << 20);
