@@ -426,13 +426,14 @@ flagcxResult_t screenTypes(int dtype, int weightDtype) {
   return flagcxSuccess;
 }
 
-constexpr size_t kMaxExtent = 0x7fffffe0;   // also when rounded up to 32
+constexpr size_t kMaxExtent = 0x7fffffff;
+constexpr size_t kMaxGradCols = 1u << 28;    // dweight's join has eight threads a column, and a launch less than 2^32
 constexpr uint32_t kFewRows = 512;
 constexpr uint64_t kStreamBytes = 32u << 20, kGradStreamBytes = 128u << 20;
 
 // One launch for every kRowsAtATime rows, `per` of them to a workgroup: the runtime
-// takes at most 2^32 threads.
-constexpr uint32_t kRowsAtATime = 1u << 22;
+// takes less than 2^32 threads.
+constexpr uint32_t kRowsAtATime = 1u << 21;
 template <class K, class A>
 flagcxResult_t launchByRow(K kernel, A a, uint32_t per, uint32_t threads, hipStream_t s) {
   const uint32_t rows = a.rows;
@@ -555,7 +556,7 @@ int fx_reduce_norm(void *out, float *scale, void *total, const void *const *in, 
   const fxNormStrides st = strides ? *strides : fxNormStrides{cols, cols, cols, cols, groups};
   if (st.in < cols || st.out < cols || (residual && st.residual < cols) || (total && st.total < cols) || (quant && st.scale < groups))
     return flagcxInvalidArgument;
-  if (!at(out, quant ? 1 : es) || (total && !at(total, es)) || (residual && !at(residual, es)) ||
+  if (!at(out, quant ? 1 : es) || total == out || (total && !at(total, es)) || (residual && !at(residual, es)) ||
       (weight && !at(weight, elementSize(weight_dtype))) || (quant && !at(scale, 4)))
     return flagcxInvalidArgument;
   NormArgs a;
@@ -590,7 +591,7 @@ int fx_reduce_norm(void *out, float *scale, void *total, const void *const *in, 
 
 size_t fx_reduce_norm_grad_workspace(size_t rows, size_t cols) {
   if (rows == 0 || cols == 0) return 0;
-  if (rows > kMaxExtent || cols > kMaxExtent) return 0;
+  if (rows > kMaxExtent || cols > kMaxGradCols) return 0;
   return ((size_t)gradParts(rows, cols) * partialStride(cols) + (cols > kGradHeld ? rows : 0)) * sizeof(float);
 }
 
@@ -599,7 +600,7 @@ int fx_reduce_norm_grad(void *dx, void *dweight, const void *dy, const void *x, 
                         void *workspace, size_t workspace_bytes, void *stream) {
   const flagcxResult_t rc = screenTypes(dtype, weight_dtype);
   if (rc != flagcxSuccess) return rc;
-  if (rows > kMaxExtent || cols > kMaxExtent || !(eps >= 0.f)) return flagcxInvalidArgument;
+  if (rows > kMaxExtent || cols > kMaxGradCols || !(eps >= 0.f)) return flagcxInvalidArgument;
   if (cols == 0 || (!dx && !dweight)) return flagcxSuccess;
   const size_t es = elementSize(dtype);
   if (dweight && !at(dweight, elementSize(weight_dtype))) return flagcxInvalidArgument;

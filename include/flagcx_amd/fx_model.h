@@ -45,7 +45,8 @@ extern "C" {
  * ceil(cols / 128) per row) is required; otherwise scale must be NULL.  A NaN
  * in a group makes its scale and all its values NaN.
  * total and out may each equal an input or the residual exactly (same stride,
- * same element size); any other overlap is undefined.  k <= FX_MAX_INPUTS (64).
+ * same element size), but not each other; any other overlap is undefined.
+ * k <= FX_MAX_INPUTS (64); rows and cols < 2^31.
  */
 typedef struct fxNormStrides {
   size_t in, residual, total, out, scale; /* elements from row to row */
@@ -66,7 +67,8 @@ int fx_reduce_norm(void *out, float *scale, void *total,
  * dx is the gradient of every in[p] and of the residual alike.  dx or dweight
  * (weight_dtype) may be NULL: not computed.  Sums run in fp32 in an order that
  * depends on the sizes alone, so equal calls give equal bits.  dx may equal dy
- * or dtotal exactly.  With rows = 0 dweight is filled with zeros.
+ * or dtotal exactly.  With rows = 0 dweight is filled with zeros.  rows < 2^31,
+ * cols <= 2^28.
  * `workspace` (device memory, 16-byte aligned, at least
  * fx_reduce_norm_grad_workspace(rows, cols) bytes) is needed when dweight is
  * asked for; it holds nothing between calls, and calls that may run at the same
@@ -97,6 +99,8 @@ int fx_reduce_norm_grad(void *dx, void *dweight, const void *dy, const void *x,
  * offsets[0] or from offsets[experts] on are left as they were.  offsets = NULL
  * with experts = 1: all rows, the plain product.
  * dtype (x, w): bf16 or fp16; out_dtype: dtype or fp32.  y overlaps nothing else.
+ * Extents and experts < 2^31.  Calls that would need 2^32 threads in one launch are
+ * not supported (9): 2^28 columns or more for few rows, 2^36 elements or more of y.
  */
 enum { FX_WEIGHT_NK = 0, FX_WEIGHT_KN = 1 };
 typedef struct fxProductStrides {

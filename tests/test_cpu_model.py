@@ -17,7 +17,7 @@ OK, BAD, NOT = N.SUCCESS, N.INVALID_ARGUMENT, N.NOT_SUPPORTED
 
 
 def norm(**kw):
-    a = dict(out=P, ins=[P, P], weight=P, rows=4, cols=256, dtype=N.DT_BF16, eps=1e-6, residual=P, total=P)
+    a = dict(out=P, ins=[P, P], weight=P, rows=4, cols=256, dtype=N.DT_BF16, eps=1e-6, residual=P, total=2 * P)
     a.update(kw)
     return K.reduce_norm(**a)
 
@@ -39,6 +39,7 @@ def test_norm_refusals():
     assert norm(out_dtype=N.DT_E4M3, scale=P, strides={**wide, "scale": 1}) == BAD
     assert norm(rows=1 << 31) == BAD and norm(cols=1 << 31) == BAD
     assert norm(rows=0, out=None, ins=[None]) == OK and norm(cols=0, out=None) == OK
+    assert norm(total=P, out=P) == BAD and norm(total=P, out=P, ins=[P]) == BAD   # one buffer for two results
 
 
 def grad(**kw):
@@ -57,7 +58,8 @@ def test_norm_gradient_refusals():
     rows = dict(dy=256, x=256, dtotal=256, dx=256)
     for name in rows:
         assert grad(strides={**rows, name: 255}) == BAD
-    assert grad(rows=1 << 31) == BAD
+    assert grad(rows=1 << 31) == BAD and grad(cols=(1 << 28) + 1, strides=None, workspace_bytes=1 << 50) == BAD
+    assert K.reduce_norm_grad_workspace(1, (1 << 28) + 1) == 0 and K.reduce_norm_grad_workspace(1, 1 << 28) > 0
     assert grad(dx=None, dweight=None, dy=None) == OK and grad(cols=0) == OK
     assert grad(rows=0, dweight=None, dy=None, x=None) == OK
     assert K.reduce_norm_grad_workspace(0, 256) == 0 and K.reduce_norm_grad_workspace(5, 0) == 0

@@ -495,3 +495,19 @@ def test_infinities_and_nan_stay_in_their_rows(dev):
         assert np.isnan(y[rows // 2 + 1:, 7]).all()
         rest = np.delete(y, [rows // 2, rows // 2 + 1], axis=0)
         assert np.isfinite(rest[:rows // 2]).all() and np.isfinite(np.delete(rest, 7, axis=1)).all()
+
+
+@pytest.mark.parametrize("nk", [True, False])
+@pytest.mark.parametrize("rows,n,k", [(8, 136, 264), (300, 264, 136), (301, 261, 133)])
+def test_fp16_subnormals_keep_their_values(dev, nk, rows, n, k):
+    """Rows of nothing but subnormal values: the products are those of the values, not of zeros."""
+    rng = np.random.default_rng(rows)
+    x = (rng.integers(1, 0x400, (rows, k)) | rng.integers(0, 2, (rows, k)) << 15).astype(np.uint16)
+    w = R.normal(N.DT_FP16, (1, n, k) if nk else (1, k, n), 5)
+    with DevBufs(dev) as b:
+        dx, dw, dy = b.put(x), b.put(w), b.alloc(rows * n * 4)
+        N.check(K.expert_product(dy, dx, dw, None, 1, rows, n, k, N.DT_FP16, out_dtype=N.DT_FP32, layout=K.W_NK if nk else K.W_KN))
+        dev.sync()
+        y = dev.to_host(dy, rows * n, np.float32).reshape(rows, n).astype(np.float64)
+    want, mag = R.product(R.codes_to_f64(x, N.DT_FP16), R.codes_to_f64(w, N.DT_FP16), [0, rows], nk)
+    assert (np.abs(y - want) <= R.rounding(want, N.DT_FP32) * 1.01 + R.sum_bound(k, mag)).all()
