@@ -303,6 +303,18 @@ __device__ __forceinline__ f32x4 mma8(const u32x4 (&n)[2], const u32x4 (&m)[2]) 
   return c;
 }
 
+// 16 bytes without the first `bytes` of them, moved to the front; zeros behind.
+__device__ __forceinline__ u32x4 dropFront(u32x4 v, uint32_t bytes) {
+  uint32_t w[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int b = 1; b < 4; b <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = (bytes >> 2 & b) ? (j + b < 4 ? w[j + b] : 0u) : w[j];
+#pragma unroll
+  for (int j = 0; j < 4; j++) v[j] = bytes >= 16 ? 0u : __builtin_amdgcn_alignbyte(j < 3 ? w[j < 3 ? j + 1 : 3] : 0u, w[j], bytes & 3);
+  return v;
+}
+
 // N consecutive columns of one output row
 template <class Out, int N>
 __device__ __forceinline__ void storeRun(Out *p, uint32_t c, uint32_t cols, const float (&f)[N]) {
@@ -473,25 +485,128 @@ struct Product {
     }
   }
 
-  // m-side scales of slab s for this lane's rows, times the n side's block scale.
+  // m-side scales of slab s for this lane's rows, and the n side's block scale.
   // A wavefront's 64 columns lie in one block of 128; columns and rows that do not
   // exist take an existing scale (their products are not stored).
-  __device__ __forceinline__ void scales(const ProductArgs &a, const Tile &t, uint32_t s, float (&out)[FM]) const {
+  __device__ __forceinline__ void scales(const ProductArgs &a, const Tile &t, uint32_t s, float (&rows)[FM], float &block) const {
     if constexpr (kScaled) {
       static_assert(TN == 64, "one block scale per wavefront");
       const uint32_t last = (a.n - 1) / FX_SCALE_GROUP, b = (t.n0 + wn) / FX_SCALE_GROUP;
-      const float sn = a.sn[(size_t)t.expert * a.expertSn + (size_t)(b < last ? b : last) * a.ldsn + s];
+      block = a.sn[(size_t)t.expert * a.expertSn + (size_t)(b < last ? b : last) * a.ldsn + s];
 #pragma unroll
       for (int q = 0; q < FM; q++) {
         const uint32_t m = t.m0 + wm + 16 * q + i;
-        out[q] = sn * a.sm[(size_t)(m < t.mEnd ? m : t.mEnd - 1) * a.ldsm + s];
+        rows[q] = a.sm[(size_t)(m < t.mEnd ? m : t.mEnd - 1) * a.ldsm + s];
       }
     }
   }
 };
 
-// Any alignment and any sizes: chunks go through registers, and the next slab's
-// are on their way while this one is multiplied.
+// Any alignment and any sizes: chunks go through registers, and the next slab's are on
+// their way while this one is multiplied.  No branch stands between the loads: a
+// chunk that a row ends in, or that lies behind its end, is loaded from the row's last
+// whole chunk and shifted into place on its way to LDS, and rows that do not exist
+// are loaded from the last one that does; of these, only what lies behind the end of
+// the reduction has to become zeros (the rest meets no result that is stored).
+// 16384 rows of 16 experts, n = 4096: k = 4096 538 us (direct), 4100 830, 4101 986; the
+// unaligned loads bound it, a second slab on its way gained nothing.  Tiles of 64 where
+// the account below puts them ahead (1024 rows of 8 experts, 1029 x 2053: 42 -> 29 us).
+template <int R, int NT, int ES, bool ACROSS, bool NSIDE>
+struct NearSide : Side<R, NT, ES, ACROSS, NSIDE> {
+  using S = Side<R, NT, ES, ACROSS, NSIDE>;
+  const char *p[S::kLoads];       // this thread's chunks of the slab to load next
+  size_t ld, advance;             // bytes
+  uint32_t own, redLast, drop;    // redLast: reduction elements of the last slab; drop: bytes that a chunk starts too early
+  __device__ __forceinline__ void start(const char *base, size_t elements, uint32_t ownHere, uint32_t red) {
+    S::init();
+    ld = elements * ES;
+    own = ownHere;
+    redLast = red;
+    advance = ACROSS ? S::kSlab * ld : 128;
+    const int32_t c = (int32_t)(S::chunk * S::kElems), end = (int32_t)(ACROSS ? own : red) - S::kElems;
+    drop = c > end ? (uint32_t)(c - end) * ES : 0;
+#pragma unroll
+    for (int i = 0; i < S::kLoads; i++) {
+      const uint32_t r = S::row + i * S::kStep;
+      p[i] = base + (size_t)(ACROSS || r < own ? r : own - 1) * ld + S::chunk * 16 - (ACROSS ? drop : 0);
+    }
+  }
+  __device__ __forceinline__ void load(u32x4 (&v)[S::kLoads], bool last) {
+    if (last)
+#pragma unroll
+      for (int i = 0; i < S::kLoads; i++) {
+        const uint32_t r = S::row + i * S::kStep;
+        if (!ACROSS) p[i] -= drop;
+        else if (r >= redLast) p[i] -= (size_t)(r - redLast + 1) * ld;
+      }
+#pragma unroll
+    for (int i = 0; i < S::kLoads; i++) {
+      v[i] = *reinterpret_cast<const u32x4_anywhere *>(p[i]);
+      p[i] += advance;
+    }
+  }
+  __device__ __forceinline__ void store(char *lds, u32x4 (&v)[S::kLoads], bool last) const {
+    if (ACROSS ? own < R : last)
+#pragma unroll
+      for (int i = 0; i < S::kLoads; i++) v[i] = dropFront(v[i], drop);
+    if (ACROSS && last)
+#pragma unroll
+      for (int i = 0; i < S::kLoads; i++)
+        if (S::row + i * S::kStep >= redLast) v[i] = u32x4{};
+#pragma unroll
+    for (int i = 0; i < S::kLoads; i++) *reinterpret_cast<u32x4 *>(lds + (i * NT + threadIdx.x) * 16) = v[i];
+  }
+};
+
+template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW>
+__global__ void __launch_bounds__(WN *WM * 64, (__is_same(T, E4m3Exact) ? 1 : 2)) productNear(ProductArgs a) {
+  using P = Product<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>;
+  constexpr int kStage = P::kLdsN + P::kLdsM;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+  Tile t;
+  if (!(DW ? findTileDw<BN, BM>(a, &t) : findTile<BN, BM, true>(a, &t))) return;
+  P p;
+  p.init();
+  const size_t nAt = NACROSS ? (size_t)t.k0 * a.ldn + t.n0 : (size_t)t.n0 * a.ldn + t.k0;
+  const size_t mAt = MACROSS ? (size_t)t.k0 * a.ldm + t.m0 : (size_t)t.m0 * a.ldm + t.k0;
+  const uint32_t slabs = (t.kLen + P::kSlab - 1) / P::kSlab;
+  if (slabs) {
+    NearSide<BN, P::kThreads, P::ES, NACROSS, true> sn;
+    NearSide<BM, P::kThreads, P::ES, MACROSS, false> sm;
+    const uint32_t redLast = t.kLen - (slabs - 1) * P::kSlab;
+    sn.start((const char *)a.pn + (nAt + (DW ? 0 : (size_t)t.expert * a.expertN)) * P::ES, a.ldn, a.n - t.n0, redLast);
+    sm.start((const char *)a.pm + mAt * P::ES, a.ldm, t.mEnd - t.m0, redLast);
+    u32x4 vn[P::N::kLoads], vm[P::M::kLoads];
+    float rows[P::FM], block = 0.f;
+    sn.load(vn, slabs == 1);
+    sm.load(vm, slabs == 1);
+    p.scales(a, t, 0, rows, block);
+    sn.store(lds, vn, slabs == 1);
+    sm.store(lds + P::kLdsN, vm, slabs == 1);
+    for (uint32_t s = 0; s < slabs; s++) {
+      const char *now = lds + (s & 1) * kStage;
+      char *then = lds + (~s & 1) * kStage;
+      const bool more = s + 1 < slabs, last = s + 2 == slabs;
+      float scale[P::FM];
+#pragma unroll
+      for (int q = 0; q < P::FM; q++) scale[q] = P::kScaled ? rows[q] * block : 0.f;
+      __syncthreads();
+      if (more) {
+        sn.load(vn, last);
+        sm.load(vm, last);
+        p.scales(a, t, s + 1, rows, block);
+      }
+      p.slab(now, now + P::kLdsN, scale);
+      if (more) {
+        sn.store(then, vn, last);
+        sm.store(then + P::kLdsN, vm, last);
+      }
+    }
+  }
+  p.store(a, t);
+}
+
+// Rows of less than a chunk: element by element.
 template <class T, class Out, int BN, int BM, int WN, int WM, bool NACROSS, bool MACROSS, bool DW>
 __global__ void __launch_bounds__(WN *WM * 64) productGuarded(ProductArgs a) {
   using P = Product<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>;
@@ -523,8 +638,10 @@ __global__ void __launch_bounds__(WN *WM * 64) productGuarded(ProductArgs a) {
   };
   if (slabs) load(0);
   for (uint32_t s = 0; s < slabs; s++) {
-    float scale[P::FM];
-    p.scales(a, t, s, scale);
+    float scale[P::FM], rows[P::FM], block = 0.f;
+    p.scales(a, t, s, rows, block);
+#pragma unroll
+    for (int q = 0; q < P::FM; q++) scale[q] = P::kScaled ? rows[q] * block : 0.f;
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < P::N::kLoads; q++) *reinterpret_cast<u32x4 *>(ln + (q * P::kThreads + threadIdx.x) * 16) = vn[q];
@@ -926,7 +1043,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t bufferAt(const void *p) {
   return __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)u, 0, 0x7fffffff, 0x00020000);
 }
 
-template <class T, int RN, int FM, int NW, int U>
+// ODD: rows at any byte.  Loads that are not a multiple of four bytes from the start
+// of memory's words run at half the rate, so the words that hold a chunk are loaded,
+// a fifth one where it ends in one, and shifted before they are multiplied (4 rows
+// each of 16 experts, 2053 x 2053: 53 -> 32 us; 2048 x 2048: 24).
+template <class T, int RN, int FM, int NW, int U, bool ODD>
 struct Thin {
   static constexpr int ES = kBytes<T>, kElems = 16 / ES;
   static constexpr bool kScaled = ES == 1;
@@ -934,7 +1055,9 @@ struct Thin {
   struct Batch {
     u32x4 w[U][RN][2], x[U][FM][2];
     float sx[U][FM], sb[U][RN];
+    float wEnd[ODD ? U : 1][RN][2], xEnd[ODD ? U : 1][FM][2];   // bits of the fifth words
   };
+  uint32_t wEndAt[RN], xEndAt[FM], wShift[RN], xShift[FM];
   f32x4 acc[RN][FM];
   __amdgpu_buffer_rsrc_t bw, bx, bs, bb;
   uint32_t ow[RN], ox[FM], os[FM], ob[RN];
@@ -953,6 +1076,12 @@ struct Thin {
         for (int r = 0; r < RN; r++) b.w[u][r][h] = loadRaw16(bw, (ow[r] + h * 64) | out, s * 128);
 #pragma unroll
         for (int f = 0; f < FM; f++) b.x[u][f][h] = loadRaw16(bx, (ox[f] + h * 64) | out, s * 128);
+        if constexpr (ODD) {
+#pragma unroll
+          for (int r = 0; r < RN; r++) b.wEnd[u][r][h] = loadRaw4(bw, (wEndAt[r] + h * 64) | out, s * 128);
+#pragma unroll
+          for (int f = 0; f < FM; f++) b.xEnd[u][f][h] = loadRaw4(bx, (xEndAt[f] + h * 64) | out, s * 128);
+        }
       }
       if constexpr (kScaled) {
 #pragma unroll
@@ -962,27 +1091,47 @@ struct Thin {
       }
     }
   }
+  __device__ __forceinline__ static u32x4 shifted(u32x4 v, float end, uint32_t bytes) {
+    const uint32_t e = __builtin_bit_cast(uint32_t, end);
+    u32x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] = __builtin_amdgcn_alignbyte(j < 3 ? v[j < 3 ? j + 1 : 3] : e, v[j], bytes);
+    return o;
+  }
   __device__ __forceinline__ void multiply(const Batch &b) {
 #pragma unroll
-    for (int u = 0; u < U; u++)
+    for (int u = 0; u < U; u++) {
+      u32x4 w[RN][2], x[FM][2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int r = 0; r < RN; r++) w[r][h] = ODD ? shifted(b.w[u][r][h], b.wEnd[ODD ? u : 0][r][h], wShift[r]) : b.w[u][r][h];
+#pragma unroll
+        for (int f = 0; f < FM; f++) x[f][h] = ODD ? shifted(b.x[u][f][h], b.xEnd[ODD ? u : 0][f][h], xShift[f]) : b.x[u][f][h];
+      }
 #pragma unroll
       for (int f = 0; f < FM; f++)
 #pragma unroll
         for (int r = 0; r < RN; r++) {
           if constexpr (kScaled) {
-            const f32x4 p = mma8<E4m3Exact>(b.w[u][r], b.x[u][f]);
+            const f32x4 p = mma8<E4m3Exact>(w[r], x[f]);
             const float sc = b.sx[u][f] * b.sb[u][r];
 #pragma unroll
             for (int v = 0; v < 4; v++) acc[r][f][v] = __builtin_fmaf(p[v], sc, acc[r][f][v]);
           } else {
 #pragma unroll
-            for (int h = 0; h < 2; h++) acc[r][f] = mma<T>(b.w[u][r][h], b.x[u][f][h], acc[r][f]);
+            for (int h = 0; h < 2; h++) acc[r][f] = mma<T>(w[r][h], x[f][h], acc[r][f]);
           }
         }
+    }
   }
-  // 16 bytes of a row from element c on, of which `cols` exist
+  // 16 bytes of a row from element c on, of which `cols` exist: from the row's last 16, shifted into place.
   __device__ __forceinline__ static u32x4 part(const char *row, uint32_t c, uint32_t cols) {
     u32x4 v = {};
+    if (cols >= (uint32_t)kElems) {
+      const uint32_t from = c < cols - kElems ? c : cols - kElems;
+      return dropFront(*reinterpret_cast<const u32x4_anywhere *>(row + (size_t)from * ES), (c - from) * ES);
+    }
 #pragma unroll
     for (int j = 0; j < kElems; j++)
       if (c + j < cols) {
@@ -998,13 +1147,23 @@ struct Thin {
     turn = full ? (t.n0 / (16 * RN) * 37 + t.expert * 11) % full : 0;
     const char *w0 = (const char *)a.pn + ((size_t)t.expert * a.expertN + (size_t)t.n0 * a.ldn) * ES;
     const char *x0 = (const char *)a.pm + (size_t)t.m0 * a.ldm * ES;
-    bw = bufferAt(w0);
-    bx = bufferAt(x0);
+    const uint32_t w3 = ODD ? (uint32_t)(uintptr_t)w0 & 3 : 0, x3 = ODD ? (uint32_t)(uintptr_t)x0 & 3 : 0;
+    bw = bufferAt(w0 - w3);
+    bx = bufferAt(x0 - x3);
 #pragma unroll
-    for (int r = 0; r < RN; r++)
-      ow[r] = t.n0 + 16 * r + i < a.n ? (uint32_t)((16 * r + i) * a.ldn * ES) + g * 16 : kOutside;
+    for (int r = 0; r < RN; r++) {
+      ow[r] = t.n0 + 16 * r + i < a.n ? (uint32_t)((16 * r + i) * a.ldn * ES) + g * 16 + w3 : kOutside;
+      wShift[r] = ow[r] & 3;
+      ow[r] &= ~3u;
+      wEndAt[r] = wShift[r] ? ow[r] + 16 : kOutside;
+    }
 #pragma unroll
-    for (int f = 0; f < FM; f++) ox[f] = 16 * f + i < own ? (uint32_t)((16 * f + i) * a.ldm * ES) + g * 16 : kOutside;
+    for (int f = 0; f < FM; f++) {
+      ox[f] = 16 * f + i < own ? (uint32_t)((16 * f + i) * a.ldm * ES) + g * 16 + x3 : kOutside;
+      xShift[f] = ox[f] & 3;
+      ox[f] &= ~3u;
+      xEndAt[f] = xShift[f] ? ox[f] + 16 : kOutside;
+    }
     const float *s0 = nullptr, *b0 = nullptr;
     if constexpr (kScaled) {
       s0 = a.sm + (size_t)t.m0 * a.ldsm;
@@ -1030,8 +1189,8 @@ struct Thin {
     }
     // what is left behind the whole slabs: one wavefront, element by element
     if (a.k % kSlab && wave == full % NW) {
-      Thin<T, RN, FM, NW, 1> last;
-      typename Thin<T, RN, FM, NW, 1>::Batch e;
+      Thin<T, RN, FM, NW, 1, false> last;
+      typename Thin<T, RN, FM, NW, 1, false>::Batch e;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const uint32_t c = full * kSlab + (h * 4 + g) * kElems;
@@ -1063,7 +1222,7 @@ struct Thin {
 
 // FM = 4 holds three bodies, for 16, 32 and 64 rows: what of a tile exists is
 // known on the device only.
-template <class T, class Out, int RN, int FM, int NW, int U>
+template <class T, class Out, int RN, int FM, int NW, int U, bool ODD>
 __global__ void __launch_bounds__(NW * 64) productThin(ProductArgs a) {
   __shared__ f32x4 lds[NW][RN * FM][64];
   Tile t;
@@ -1072,7 +1231,7 @@ __global__ void __launch_bounds__(NW * 64) productThin(ProductArgs a) {
   const uint32_t own = t.mEnd - t.m0, live = own >= 16 * FM ? FM : (own + 15) / 16;
   auto body = [&](auto rows) {
     constexpr int F = decltype(rows)::value;
-    Thin<T, RN, F, NW, (F == FM ? U : F == 1 ? 4 * U : 2 * U)> p;
+    Thin<T, RN, F, NW, (F == FM ? U : F == 1 ? 4 * U : 2 * U), ODD> p;
     p.run(a, t, wave, i, g);
 #pragma unroll
     for (int r = 0; r < RN; r++)
@@ -1121,18 +1280,23 @@ inline flagcxResult_t launchGrid(const void *kernel, ProductArgs &a, uint32_t bn
   return hipLaunchKernel(kernel, dim3((uint32_t)grid), dim3(threads), argv, 0, s) == hipSuccess ? flagcxSuccess : flagcxUnhandledDeviceError;
 }
 
-// SN = 0: guarded
+// SN = 1: any alignment; SN = 0: rows of less than a chunk
 template <class T, class Out, int BN, int BM, int WN, int WM, int SN, int SM, bool NACROSS, bool MACROSS, bool DW, bool TOUCH = false>
 flagcxResult_t launchTiles(ProductArgs a, hipStream_t s) {
   const void *kernel;
-  if constexpr (SN != 0) kernel = reinterpret_cast<const void *>(productDirect<T, Out, BN, BM, WN, WM, SN, SM, NACROSS, MACROSS, DW, TOUCH>);
+  if constexpr (SN == 1) kernel = reinterpret_cast<const void *>(productNear<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
+  else if constexpr (SN != 0) kernel = reinterpret_cast<const void *>(productDirect<T, Out, BN, BM, WN, WM, SN, SM, NACROSS, MACROSS, DW, TOUCH>);
   else kernel = reinterpret_cast<const void *>(productGuarded<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
   return launchGrid(kernel, a, BN, BM, DW, WN * WM * 64, s);
 }
 
 template <class T, class Out, int RN, int FM, int NW, int U>
 flagcxResult_t launchThin(ProductArgs a, hipStream_t s) {
-  return launchGrid(reinterpret_cast<const void *>(productThin<T, Out, RN, FM, NW, U>), a, 16 * RN, 16 * FM, false, NW * 64, s);
+  const size_t es = kBytes<T>;
+  const bool odd = ((uintptr_t)a.pn | (uintptr_t)a.pm | a.ldn * es | a.ldm * es | a.expertN * es) & 3;
+  const void *kernel = odd ? reinterpret_cast<const void *>(productThin<T, Out, RN, FM, NW, U, true>)
+                           : reinterpret_cast<const void *>(productThin<T, Out, RN, FM, NW, U, false>);
+  return launchGrid(kernel, a, 16 * RN, 16 * FM, false, NW * 64, s);
 }
 
 // Whole 16-byte chunks everywhere: what the direct kernels assume.  `inner` is the
@@ -1212,7 +1376,13 @@ flagcxResult_t launchShapes(const ProductArgs &a, hipStream_t s) {
   }
   const bool direct = wholeChunks(a.pn, a.ldn, a.expertN, NACROSS ? a.n : a.k, es) &&
                       wholeChunks(a.pm, a.ldm, 0, MACROSS ? a.m : a.k, es) && a.ldsm < (1u << 20);
-  if (!direct) return launchTiles<T, Out, 128, 128, 2, 2, 0, 0, NACROSS, MACROSS, DW>(a, s);
+  if (!direct) {
+    const size_t inner = (NACROSS ? a.n : a.k) < (MACROSS ? a.m : a.k) ? (NACROSS ? a.n : a.k) : (MACROSS ? a.m : a.k);
+    if (inner * es < 16) return launchTiles<T, Out, 128, 128, 2, 2, 0, 0, NACROSS, MACROSS, DW>(a, s);
+    if (cheapestTile(a, DW, es, es == 1 ? kCost8 : kCost16, kTile128) != kTile128)
+      return launchTiles<T, Out, 64, 64, 1, 2, 1, 1, NACROSS, MACROSS, DW>(a, s);
+    return launchTiles<T, Out, 128, 128, 2, 2, 1, 1, NACROSS, MACROSS, DW>(a, s);
+  }
   // widened e4m3 operands leave no registers for the largest tile
   constexpr bool kLargest = !__is_same(T, E4m3Exact);
   switch (cheapestTile(a, DW, es, es == 1 ? kCost8 : kCost16, kLargest ? kTile256 : kTile128)) {

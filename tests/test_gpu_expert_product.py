@@ -511,3 +511,50 @@ def test_fp16_subnormals_keep_their_values(dev, nk, rows, n, k):
         y = dev.to_host(dy, rows * n, np.float32).reshape(rows, n).astype(np.float64)
     want, mag = R.product(R.codes_to_f64(x, N.DT_FP16), R.codes_to_f64(w, N.DT_FP16), [0, rows], nk)
     assert (np.abs(y - want) <= R.rounding(want, N.DT_FP32) * 1.01 + R.sum_bound(k, mag)).all()
+
+
+@pytest.mark.parametrize("rest", [1, 2, 3, 5, 7, 8, 9, 11, 15, 16, 17, 31, 33, 63])
+def test_reductions_and_widths_of_every_remainder(dev, rest):
+    """What is left behind whole chunks and whole slabs, on rows that start at any byte: few rows, small and large tiles."""
+    rng = np.random.default_rng(rest)
+    n, k = 128 + rest, 192 + rest
+    for nk in (True, False):
+        run(dev, N.DT_BF16, 21, n, k, ragged(21, 3, rng), nk=nk, seed=rest)
+        run(dev, N.DT_FP16, 500, n, k, ragged(500, 3, rng), nk=nk, out32=True, seed=rest)
+        run(dev, N.DT_FP16, 150, rest, rest, None, nk=nk, seed=rest)
+    run_dw(dev, N.DT_BF16, 300, n, k, ragged(300, 3, rng), seed=rest)
+    run_dw(dev, N.DT_FP16, 60 + rest, rest, n, ragged(60 + rest, 2, rng), out32=True, seed=rest)
+    run8(dev, 21, n, k, ragged(21, 3, rng), N.DT_BF16, seed=rest)
+    run8(dev, 500, n, k, ragged(500, 3, rng), N.DT_FP16, seed=rest)
+    run8(dev, 500, n, k, ragged(500, 3, rng), N.DT_FP32, shift=rest % 4, pad=rest % 5, seed=rest)
+    run8(dev, 150, rest, rest, None, N.DT_BF16, seed=rest)
+
+
+def test_large_products_of_odd_sizes(dev):
+    """Enough rows for tiles of 128 at sizes that no vector divides."""
+    rng = np.random.default_rng(9)
+    for rows, n, k in ((4500, 2057, 141), (4501, 2061, 322)):
+        for nk in (True, False):
+            for t in (N.DT_BF16, N.DT_FP16):
+                run(dev, t, rows, n, k, ragged(rows, 3, rng), nk=nk, out32=rows % 2 == 0, seed=n)
+                run(dev, t, rows, n, k, None, nk=nk, out32=rows % 2 == 1, seed=n)
+        for out in (N.DT_BF16, N.DT_FP16, N.DT_FP32):
+            run8(dev, rows, n, k, ragged(rows, 3, rng), out, seed=n)
+    for t in (N.DT_BF16, N.DT_FP16):
+        for out32 in (False, True):
+            run_dw(dev, t, 1501, 1029, 2053, ragged(1501, 12, rng), out32=out32, seed=3)
+
+
+@pytest.mark.parametrize("nk", [True, False])
+def test_rows_of_less_than_a_chunk_and_few_rows_at_any_byte(dev, nk):
+    rng = np.random.default_rng(4)
+    for t in (N.DT_BF16, N.DT_FP16):
+        for out32 in (False, True):
+            run(dev, t, 150, 5, 7, None, nk=nk, out32=out32, seed=1)
+            run(dev, t, 31, 205, 203, ragged(31, 1, rng), nk=nk, out32=out32, seed=2)
+            run(dev, t, 20, 205, 203, None, nk=nk, out32=out32, pad=1, shift=1, seed=3)
+            run_dw(dev, t, 150, 5, 70, ragged(150, 3, rng), out32=out32, seed=4)
+    for out in (N.DT_BF16, N.DT_FP16, N.DT_FP32):
+        run8(dev, 150, 70, 13, None, out, seed=5)
+        run8(dev, 50, 205, 203, None, out, seed=6)
+        run8(dev, 18, 205, 403, ragged(18, 1, rng), out, pad=1, shift=3, seed=7)
