@@ -1,5 +1,6 @@
 """Python-side callers of the kernel C ABI (pointers are plain integers)."""
 import ctypes as C
+import functools
 
 import numpy as np
 
@@ -8,8 +9,13 @@ from . import _native as N
 lib = N.lib
 
 
+@functools.lru_cache(maxsize=256)
+def _pointers(n):
+    return C.c_void_p * n
+
+
 def _ptr_array(ptrs):
-    return (C.c_void_p * len(ptrs))(*ptrs)
+    return _pointers(len(ptrs))(*ptrs)
 
 
 def reduce_copy(out, ins, count, dtype, op, first=0, stream=None):
