@@ -16,7 +16,7 @@
 // exchanged by a function of the row, so that the eight lanes that a 128-bit read
 // serves at a time meet eight different chunks.  An "across" tile keeps its rows
 // of the reduction and is read with the transposing LDS loads, four rows by 32
-// bytes at a time; its 32-byte units are exchanged by the row's two low bits.
+// bytes at a time; its 32-byte units are exchanged by a function of the row.
 #pragma once
 #include "flagcx_amd/fx_model.h"
 #include "fx_vec.hpp"
@@ -209,6 +209,14 @@ __device__ __forceinline__ uint32_t exchange(uint32_t r) {
   return NSIDE ? ((r & 3) | ((r >> 1) & 4)) : (r & 7);
 }
 
+// Unit exchange of an "across" tile whose rows span all 64 banks: by the row's two low
+// bits, so that the four rows of a transposing load meet different banks, and by its
+// fourth, so that two lane groups, eight rows apart, do.
+template <int R>
+__device__ __forceinline__ uint32_t exchangeUnits(uint32_t row) {
+  return (row & 3) | (R >= 128 ? (row >> 1) & 4 : 0);
+}
+
 // R = extent of the tile in its own index, NT = threads, ES = bytes per element.
 template <int R, int NT, int ES, bool ACROSS, bool NSIDE>
 struct Side {
@@ -218,14 +226,14 @@ struct Side {
   static constexpr int kElems = 16 / ES;
   static constexpr uint32_t kSlab = 128 / ES;            // reduction elements per slab
 
-  static_assert(kStep % (ACROSS ? 4 : 16) == 0, "a thread's chunks lie in rows that the exchange treats alike");
+  static_assert(kStep % 16 == 0, "a thread's chunks lie in rows that the exchange treats alike");
 
   // position of this thread's first chunk
   uint32_t row, chunk;
   __device__ __forceinline__ void init() {
     row = threadIdx.x / kPerRow;
     const uint32_t p = threadIdx.x % kPerRow;
-    chunk = ACROSS ? ((((p >> 1) ^ (row & 3)) << 1) | (p & 1)) : (p ^ exchange<NSIDE>(row));
+    chunk = ACROSS ? ((((p >> 1) ^ exchangeUnits<R>(row)) << 1) | (p & 1)) : (p ^ exchange<NSIDE>(row));
   }
 
   // One chunk, element by element where it is not whole; `base` = the tile's own
@@ -262,7 +270,7 @@ __device__ __forceinline__ u32x4 readAcross(const char *lds, uint32_t wave0, int
   typedef __attribute__((address_space(3))) s16x4 *lds64;
   const uint32_t unit = (wave0 + 16 * f) / 16;
   const uint32_t k = 32 * half + 8 * g + (i >> 2);
-  const uint32_t at = k * (R * 2) + ((unit ^ (i >> 2)) * 32) + (i & 3) * 8;
+  const uint32_t at = k * (R * 2) + ((unit ^ exchangeUnits<R>(k)) * 32) + (i & 3) * 8;
   const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds64)(lds + at));
   const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds64)(lds + at + 4 * R * 2));
   const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
@@ -705,17 +713,15 @@ struct DirectSide : Side<R, NT, ES, ACROSS, NSIDE> {
   }
 };
 
-// The e4m3 rows' scales of one slab, one float per row of the tile, brought to LDS
-// in the order in which a lane wants them (its fragments' rows side by side).  Every
-// wavefront issues one load, also those without a row, so that all count alike.
-template <int BM, int TM>
+// The e4m3 rows' scales of one slab, one float per row of the tile, brought to LDS.
+// Every wavefront issues one load, also those without a row, so that all count alike.
+template <int BM>
 struct DirectScales {
-  static constexpr uint32_t FM = TM / 16;
   uint32_t voff;
   uint64_t at;
   __device__ __forceinline__ void start(const float *base, size_t ld, uint32_t own) {
-    const uint32_t pos = threadIdx.x, rem = pos % TM, row = pos / TM * TM + 16 * (rem % FM) + rem / FM;
-    voff = pos < BM && row < own ? (uint32_t)(row * ld * 4) : kOutside;
+    const uint32_t row = threadIdx.x;
+    voff = row < BM && row < own ? (uint32_t)(row * ld * 4) : kOutside;
     at = (uint64_t)(uintptr_t)base;
   }
   __device__ __forceinline__ void issue(uint32_t lds, uint32_t wave, bool there) {
@@ -775,7 +781,7 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
   const uint32_t wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
   DirectSide<BN, P::kThreads, P::ES, NACROSS, true> sn;
   DirectSide<BM, P::kThreads, P::ES, MACROSS, false> sm;
-  DirectScales<BM, P::TM> ss;
+  DirectScales<BM> ss;
   const size_t nAt = NACROSS ? (size_t)t.k0 * a.ldn + t.n0 : (size_t)t.n0 * a.ldn + t.k0;
   const size_t mAt = MACROSS ? (size_t)t.k0 * a.ldm + t.m0 : (size_t)t.m0 * a.ldm + t.k0;
   sn.start((const char *)a.pn + (nAt + (DW ? 0 : (size_t)t.expert * a.expertN)) * P::ES, a.ldn, a.n - t.n0);
@@ -881,7 +887,7 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
         for (int q = 0; q < P::FM; q++) {
 #pragma unroll
           for (int h = 0; h < 2; h++) b.m[q][h] = p.readM(lm, q, h);
-          b.scale[q] = *reinterpret_cast<const float *>(lm + P::kLdsM + (p.wm + p.i * P::FM + q) * 4);
+          b.scale[q] = *reinterpret_cast<const float *>(lm + P::kLdsM + (p.wm + 16 * q + p.i) * 4);
         }
       };
       auto multiply = [&](const Slab &b, uint32_t s) {
@@ -929,7 +935,7 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
         for (int j = 0; j < 2; j++) {
           m[buffer][j][0] = p.readM(lm, 2 * pair + j, 0);
           m[buffer][j][1] = p.readM(lm, 2 * pair + j, 1);
-          scale[buffer][j] = *reinterpret_cast<const float *>(lm + P::kLdsM + (p.wm + p.i * P::FM + 2 * pair + j) * 4);
+          scale[buffer][j] = *reinterpret_cast<const float *>(lm + P::kLdsM + (p.wm + 16 * (2 * pair + j) + p.i) * 4);
         }
       };
       auto readN = [&](int f) {
