@@ -17,6 +17,11 @@
 // serves at a time meet eight different chunks.  An "across" tile keeps its rows
 // of the reduction and is read with the transposing LDS loads, four rows by 32
 // bytes at a time; its 32-byte units are exchanged by a function of the row.
+//
+// Measured: 8192^3 bf16 1.35 PFLOP/s (matrix cores about half the time busy: the rest is
+// what waits and stores cost), e4m3 2.05 to 2.2; 16384 rows of 16 experts, 4096 x 4096
+// bf16, 0.52 to 0.54 ms (1.0 PFLOP/s: experts' last tiles and weights from memory); one
+// token through 8 of 64 experts, 2048 x 4096, 26 us (5.2 TB/s of weights).
 #pragma once
 #include "flagcx_amd/fx_model.h"
 #include "fx_vec.hpp"
@@ -737,7 +742,8 @@ struct DirectScales {
 // further on, four bytes of each that nobody reads, which brings them into the die's
 // cache; neighbouring tiles share a slab's lines out among them.  Loads return in
 // order; the wait for a slab leaves the last touch out, so it has two slabs' time.
-// (8192^3 from memory 633 -> 579 us; where few tiles share weights it gains nothing.)
+// (8192^3 from memory 588 -> 543 us; 4096 rows each of 4 experts, 4096 x 4096, 352 ->
+// 339; where few tiles share weights it gains nothing.)
 constexpr uint32_t kTouchAhead = 4;
 constexpr uint32_t kTurn = 37;
 
