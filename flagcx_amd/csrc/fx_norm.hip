@@ -483,7 +483,9 @@ flagcxResult_t launchNormOut(const NormArgs &a, bool quant, hipStream_t s) {
 }
 
 // Workgroups of the gradients, each with a row of partial sums: one per compute unit
-// (8192 x 8192 bf16: 89 us, with 384 105, with 512 94); fewer when there are fewer rows.
+// (8192 x 8192 bf16: 89 us, with 384 105, with 512 94), or as many as give each the same
+// number of rows, with fewer partial sums to join (260 x 8192: 13.3 -> 11.6 us; 777 x 5003
+// fp16: 16.9 -> 16.4).
 constexpr uint32_t kGradWgs = 256;
 constexpr uint32_t kLongParts = 64;
 constexpr uint32_t kGradHeld = 1024 * 2 * 8;   // widest row that the gradients hold
@@ -493,7 +495,8 @@ bool waveRows(size_t cols) { return cols <= 64 * 2 * 8; }
 uint32_t gradParts(size_t rows, size_t cols) {
   const size_t most = cols > kGradHeld ? kLongParts : kGradWgs;
   const size_t want = waveRows(cols) ? (rows + 3) / 4 : rows;
-  return (uint32_t)(want < most ? want : most);
+  const size_t rounds = (want + most - 1) / most;
+  return (uint32_t)((want + rounds - 1) / rounds);
 }
 
 template <class T, bool STREAM>

@@ -85,7 +85,7 @@ def norm_grad(dy, x, weight, dtotal, eps):
     bx = (r * np.abs(g) + np.abs(x) * r ** 3 * np.abs(m)) * 220 * E + np.abs(x) * r ** 3 * dm + 4 * E * np.abs(dx)
     if dtotal is not None:
         bx = bx + 4 * E * np.abs(dtotal)
-    # dweight: each term is off by 80 E; rows / 256 additions in a workgroup (long rows: / 64), 3 over its wavefronts,
+    # dweight: each term is off by 80 E; rows / 256 + 1 additions in a workgroup (long rows: / 64), 3 over its wavefronts,
     # 8 + 32 where the workgroups' sums are joined: under 120 at the sizes tested here
     bw = 200 * E * np.sum(np.abs(dy * x * r), axis=0)
     return dx, dw, bx, bw
