@@ -558,3 +558,73 @@ def test_rows_of_less_than_a_chunk_and_few_rows_at_any_byte(dev, nk):
         run8(dev, 150, 70, 13, None, out, seed=5)
         run8(dev, 50, 205, 203, None, out, seed=6)
         run8(dev, 18, 205, 403, ragged(18, 1, rng), out, pad=1, shift=3, seed=7)
+
+
+def cancelling(rng, shape):
+    """e4m3 codes in which every run of eight columns holds two large values of opposite sign and six small ones, at random
+    places; used on both sides, the large products of a run cancel."""
+    rows, k = int(np.prod(shape[:-1])), shape[-1]
+    c = rng.integers(0x01, 0x40, (rows, -(-k // 8), 8)).astype(np.uint8)
+    big = rng.integers(0x70, 0x7f, (rows, c.shape[1]))
+    c[:, :, 2], c[:, :, 5] = big, big
+    return c.reshape(rows, -1)[:, :k].reshape(shape)
+
+
+def just_below(side, shape):
+    """Runs of one product 256 * 256 and seven of 2 * 3.75, just below the eighth that the cut keeps."""
+    c = np.full(shape, 0x47 if side else 0x40, np.uint8)
+    c[..., ::8] = 0x78
+    return c
+
+
+def cut_products(x, w):
+    """Sums over whole rows of k columns as the 8-bit matrix instructions form them, in 64 bits but for the cut, and the
+    magnitudes that the documented bound is taken of.  x [rows, k], w [n, k]: codes."""
+    field = lambda c: np.where(c & 0x78, ((c >> 3) & 15).astype(int) - 7, -6)  # noqa: E731
+    lifted = lambda c: np.where(c & 0x7f, np.maximum(np.abs(R.E4M3[c]), 2.0 ** -6), 0.0)  # noqa: E731
+    got, mag = np.zeros((x.shape[0], w.shape[0])), np.zeros((x.shape[0], w.shape[0]))
+    for c in range(0, x.shape[1], 8):
+        xs, ws = x[:, None, c:c + 8], w[None, :, c:c + 8]
+        p = R.E4M3[xs] * R.E4M3[ws]
+        e = np.where(p != 0, field(xs) + field(ws), -99).max(axis=2, keepdims=True)
+        u = 2.0 ** (e - 13.0)
+        got += (np.trunc(p / u) * u).sum(axis=2)
+        mag += (lifted(xs) * lifted(ws)).max(axis=2)
+    return got, mag
+
+
+@pytest.mark.parametrize("out", [N.DT_BF16, N.DT_FP16, N.DT_FP32])
+@pytest.mark.parametrize("kind", ["cancelling", "below", "any"])
+@pytest.mark.parametrize("rows,n,k", [(70, 64, 128), (200, 200, 256), (700, 72, 141), (300, 520, 13), (5000, 40, 384), (2100, 272, 128)])
+def test_e4m3_sums_are_cut_as_documented(dev, out, kind, rows, n, k):
+    """One scale of 1, so that the result is the sum itself.  16-bit results: off the exact sum by less than 2^-10 of each
+    run's largest product (a run of eight loses less than 2^(e-13) of each of its eight products at most, and the largest
+    lifted one is at least 2^e); and what the cut leaves is summed as in fp32.  fp32 results: no cut."""
+    rng = np.random.default_rng(rows)
+    some = np.array([c for c in range(256) if c & 127 != 127], np.uint8)
+    make = {"cancelling": lambda side, s: cancelling(rng, s), "below": just_below, "any": lambda side, s: rng.choice(some, s)}[kind]
+    x, w = make(0, (rows, k)), make(1, (n, k))
+    if kind == "cancelling":
+        x[:, 5::8] |= 0x80                                   # + and - in the pair
+    kg, ng = -(-k // 128), -(-n // 128)
+    odt = np.float32 if out == N.DT_FP32 else np.uint16
+    with DevBufs(dev) as b:
+        dx, dw, dy = b.put(x), b.put(w), b.alloc(rows * n * 4)
+        ones = b.put(np.ones(max(rows, ng) * kg, np.float32))
+        N.check(K.expert_product_e4m3(dy, dx, ones, dw, ones, None, 1, rows, n, k, out))
+        dev.sync()
+        got = R.codes_to_f64(dev.to_host(dy, rows * n, odt).reshape(rows, n), out)
+    want = R.E4M3[x] @ R.E4M3[w].T
+    mag = np.abs(R.E4M3[x]) @ np.abs(R.E4M3[w]).T
+    sums = R.sum_bound(min(k, 128) + kg + 4, mag)
+    if out == N.DT_FP32:
+        assert R.within(got, want, out, sums)
+        return
+    cut, largest = cut_products(x, w)
+    assert (np.abs(cut - want) <= 2.0 ** -10 * largest).all()
+    assert R.within(got, want, out, sums + 2.0 ** -10 * largest)
+    assert R.within(got, cut, out, sums)
+    if kind == "cancelling" and k % 8 == 0:                  # every pair is whole: what the documentation warns of
+        assert (np.abs(cut - want) > np.abs(want) / 4).any()
+    if kind == "below":
+        assert (np.abs(cut - want) > 2.0 ** -11 * mag).all()
