@@ -498,6 +498,17 @@ uint32_t gradParts(size_t rows, size_t cols) {
   const size_t rounds = (want + most - 1) / most;
   return (uint32_t)((want + rounds - 1) / rounds);
 }
+// What one call uses; and what every call of at most so many rows and columns can do with, for callers that keep one
+// workspace: fewer rows may well have more parts, and the widest rows that are held more than wider ones.
+size_t gradBytes(size_t rows, size_t cols) {
+  return ((size_t)gradParts(rows, cols) * partialStride(cols) + (cols > kGradHeld ? rows : 0)) * sizeof(float);
+}
+size_t gradBytesUpTo(size_t rows, size_t cols) {
+  const size_t want = waveRows(cols) ? (rows + 3) / 4 : rows;
+  const size_t held = (want < kGradWgs ? want : kGradWgs) * partialStride(cols < kGradHeld ? cols : kGradHeld);
+  const size_t wide = cols > kGradHeld ? (rows < kLongParts ? rows : kLongParts) * partialStride(cols) + rows : 0;
+  return (held > wide ? held : wide) * sizeof(float);
+}
 
 template <class T, bool STREAM>
 flagcxResult_t launchGradRows(const NormGradArgs &a, uint32_t parts, hipStream_t s) {
@@ -598,7 +609,7 @@ int fx_reduce_norm(void *out, float *scale, void *total, const void *const *in, 
 size_t fx_reduce_norm_grad_workspace(size_t rows, size_t cols) {
   if (rows == 0 || cols == 0) return 0;
   if (rows > kMaxExtent || cols > kMaxGradCols) return 0;
-  return ((size_t)gradParts(rows, cols) * partialStride(cols) + (cols > kGradHeld ? rows : 0)) * sizeof(float);
+  return gradBytesUpTo(rows, cols);
 }
 
 int fx_reduce_norm_grad(void *dx, void *dweight, const void *dy, const void *x, const void *dtotal, const void *weight,
@@ -616,7 +627,7 @@ int fx_reduce_norm_grad(void *dx, void *dweight, const void *dy, const void *x, 
         (weight && !at(weight, elementSize(weight_dtype))))
       return flagcxInvalidArgument;
     if (st.dy < cols || st.x < cols || (dtotal && st.dtotal < cols) || (dx && st.dx < cols)) return flagcxInvalidArgument;
-    if (dweight && (!at(workspace, 16) || workspace_bytes < fx_reduce_norm_grad_workspace(rows, cols)))
+    if (dweight && (!at(workspace, 16) || workspace_bytes < gradBytes(rows, cols)))
       return flagcxInvalidArgument;
   }
   NormGradArgs a;

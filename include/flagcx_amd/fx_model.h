@@ -69,9 +69,11 @@ int fx_reduce_norm(void *out, float *scale, void *total,
  * depends on the sizes alone, so equal calls give equal bits.  dx may equal dy
  * or dtotal exactly.  With rows = 0 dweight is filled with zeros.  rows < 2^31,
  * cols <= 2^28.
- * `workspace` (device memory, 16-byte aligned, at least
- * fx_reduce_norm_grad_workspace(rows, cols) bytes) is needed when dweight is
- * asked for; it holds nothing between calls, and calls that may run at the same
+ * `workspace` (device memory, 16-byte aligned) is needed when dweight is asked
+ * for.  fx_reduce_norm_grad_workspace(rows, cols) bytes do for every call of at
+ * most that many rows and at most that many columns, so one workspace sized for
+ * the largest serves them all; a call refuses one that is smaller than what it
+ * uses itself.  It holds nothing between calls, and calls that may run at the same
  * time need one each.
  */
 typedef struct fxNormGradStrides {

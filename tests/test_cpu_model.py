@@ -65,6 +65,21 @@ def test_norm_gradient_refusals():
     assert K.reduce_norm_grad_workspace(0, 256) == 0 and K.reduce_norm_grad_workspace(5, 0) == 0
 
 
+def test_norm_gradient_workspace_of_the_largest_call_serves_all():
+    """Never less for more rows or columns, and a call of fewer rows accepts what was sized for more."""
+    rows = list(range(1, 530)) + [700, 1023, 1024, 1025, 1029, 4095, 4096, 4097, 100000]
+    cols = [1, 31, 32, 33, 500, 1023, 1024, 1025, 1056, 4096, 8192, 8200, 16352, 16383, 16384, 16385, 16416, 17000, 40000, 65537]
+    need = [[K.reduce_norm_grad_workspace(r, c) for c in cols] for r in rows]
+    for a, b in zip(need, need[1:]):
+        assert all(x <= y for x, y in zip(a, b))
+    for a in need:
+        assert all(x <= y for x, y in zip(a, a[1:]))
+    for r, c, most in ((256, 8192, 300), (256, 8192, 257), (1, 16384, 2), (512, 16384, 512), (1000, 700, 1029)):
+        have = K.reduce_norm_grad_workspace(most, c + (c == 16384))
+        assert have >= K.reduce_norm_grad_workspace(r, c)
+    assert grad(rows=256, cols=8192, workspace_bytes=256 * 8192 * 4 - 1) == BAD        # what the call itself uses
+
+
 def product(**kw):
     a = dict(y=P, x=P, w=P, offsets=P, experts=4, rows=64, n=128, k=256, dtype=N.DT_BF16)
     a.update(kw)

@@ -333,3 +333,21 @@ def test_norm_gradients_on_two_streams_with_a_workspace_each(dev):
             assert np.array_equal(got[0], a[0]) and np.array_equal(got[1], a[1])
     for st in streams:
         dev.stream_destroy(st)
+
+
+@pytest.mark.parametrize("rows,most,cols,widest", [(256, 300, 8192, 8192), (256, 257, 5003, 5003), (512, 512, 16384, 16385),
+                                                   (1000, 1029, 700, 700), (64, 70, 20000, 33000), (3, 5000, 100, 40000)])
+def test_norm_gradients_in_the_workspace_of_a_larger_call(dev, rows, most, cols, widest):
+    t, need = N.DT_BF16, K.reduce_norm_grad_workspace(most, widest)
+    x, dy, w = R.normal(t, (rows, cols), 1, 2.0), R.normal(t, (rows, cols), 2), R.normal(t, (cols,), 3)
+    with DevBufs(dev) as b:
+        ws = b.put(np.full(need + 64, 0xEE, np.uint8))
+        dx, dw = b.alloc(rows * cols * 2), b.alloc(cols * 2)
+        N.check(K.reduce_norm_grad(dx, dw, b.put(dy), b.put(x), b.put(w), rows, cols, t, ws, need, eps=EPS), "fx_reduce_norm_grad")
+        dev.sync()
+        gx = R.codes_to_f64(dev.to_host(dx, rows * cols, np.uint16).reshape(rows, cols), t)
+        gw = R.codes_to_f64(dev.to_host(dw, cols, np.uint16), t)
+        assert (dev.to_host(ws, need + 64, np.uint8)[need:] == 0xEE).all()
+    f = lambda a: R.codes_to_f64(a, t)  # noqa: E731
+    edx, edw, bx, bw = R.norm_grad(f(dy), f(x), f(w), None, EPS)
+    assert (np.abs(gx - edx) <= R.rounding(edx, t) * 1.01 + bx).all() and (np.abs(gw - edw) <= R.rounding(edw, t) * 1.01 + bw).all()
