@@ -252,7 +252,7 @@ def run_norm(dev, a):
     es, rmax = N.DTYPE_SIZE[dtype], size(a.max)
     ins = [_normal(dev, rmax * c, dtype, p) for p in range(k)]
     res, w = _normal(dev, rmax * c, dtype, 90), _normal(dev, c, dtype, 91)
-    tot, out, scale = (dev.malloc(rmax * c * es) for _ in range(3))
+    tot, out, scale = dev.malloc(rmax * c * es), dev.malloc(rmax * c * es), dev.malloc(4 * rmax * -(-c // 128))
     space = K.reduce_norm_grad_workspace(rmax, c)
     ws, dw = dev.malloc(space + 64), dev.malloc(c * es)
     r = size(a.min)

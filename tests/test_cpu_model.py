@@ -1,5 +1,6 @@
 """The operators behind the collectives without a GPU: what they refuse, what they
 accept as nothing to do, and the gradients' formulas against differences."""
+import argparse
 import os
 import re
 import shutil
@@ -10,6 +11,7 @@ import pytest
 
 from flagcx_amd import _native as N
 from flagcx_amd import kernels as K
+from flagcx_amd import perf
 from tests import model_ref as R
 
 P = 0x1000
@@ -199,3 +201,58 @@ def test_stride_blocks_match_the_header():
         body = re.search(r"typedef struct %s \{(.*?)\}" % name, text, re.S).group(1)
         fields = re.findall(r"\w+", body.replace("size_t", ""))
         assert [f.rstrip("_") for f, _ in cls._fields_] == fields, name
+
+
+class Buffers:
+    """Stands in for a device: hands out address ranges and answers how much of one is left behind an address."""
+
+    def __init__(self):
+        self.at, self.sizes = 1 << 20, {}
+
+    def malloc(self, n):
+        p = self.at
+        self.sizes[p] = n
+        self.at += (n + (1 << 20)) & ~0xfff
+        return p
+
+    def upload(self, p, a):
+        assert a.nbytes <= self.left(p)
+
+    def to_device(self, a):
+        return self.malloc(a.nbytes)
+
+    def left(self, p):
+        return next((base + n - p for base, n in self.sizes.items() if base <= p <= base + n), 0)
+
+
+@pytest.mark.parametrize("cols", [1, 7, 129, 640])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_norm_command_allocates_what_the_calls_write(monkeypatch, capsys, cols, dtype):
+    dev, es = Buffers(), 2 if dtype == "bf16" else 4
+
+    class Timer:
+        raw = None
+
+        def __init__(self, dev):
+            pass
+
+        def both(self, fn, cold):
+            fn()
+            return 1.0, None
+
+    def forward(out, ins, weight, rows, cols, dt, *, eps, residual, total, stream, scale=None, out_dtype=None):
+        n = rows * cols * es
+        assert all(dev.left(p) >= n for p in (*ins, residual, total)) and dev.left(weight) >= cols * es
+        assert dev.left(out) >= (rows * cols if scale else n)
+        assert scale is None or dev.left(scale) >= 4 * rows * -(-cols // 128)
+        return OK
+
+    def backward(dx, dw, dy, x, weight, rows, cols, dt, ws, nbytes, *, eps, dtotal, stream):
+        assert all(dev.left(p) >= rows * cols * es for p in (dx, dy, x, dtotal)) and dev.left(dw) >= cols * es
+        assert dev.left(ws) >= nbytes >= K.reduce_norm_grad_workspace(rows, cols)
+        return OK
+    monkeypatch.setattr(perf, "Timer", Timer)
+    monkeypatch.setattr(perf.K, "reduce_norm", forward)
+    monkeypatch.setattr(perf.K, "reduce_norm_grad", backward)
+    perf.run_norm(dev, argparse.Namespace(dtype=dtype, k=2, cols=cols, min="3", max="700", factor=3, cold=False))
+    assert capsys.readouterr().out.count("GB/s") == 15
