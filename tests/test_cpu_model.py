@@ -254,5 +254,5 @@ def test_norm_command_allocates_what_the_calls_write(monkeypatch, capsys, cols, 
     monkeypatch.setattr(perf, "Timer", Timer)
     monkeypatch.setattr(perf.K, "reduce_norm", forward)
     monkeypatch.setattr(perf.K, "reduce_norm_grad", backward)
-    perf.run_norm(dev, argparse.Namespace(dtype=dtype, k=2, cols=cols, min="3", max="700", factor=3, cold=False))
-    assert capsys.readouterr().out.count("GB/s") == 15
+    perf.run_norm(dev, argparse.Namespace(dtype=dtype, k=2, cols=cols, min="3", max="729", factor=3, cold=False))
+    assert capsys.readouterr().out.count("GB/s") == 18
