@@ -685,10 +685,11 @@ __global__ void __launch_bounds__(WN *WM * 64) productGuarded(ProductArgs a) {
 // The loads are issued from inline assembly (they have no register outputs): the
 // compiler does not know that they write LDS, and every read of LDS behind one
 // would otherwise wait for it.  The waits are therefore written here: a slab is
-// read only behind a wait for all of this wavefront's loads and a barrier.
+// read only behind a wait for all of this wavefront's loads and a barrier.  The LDS
+// address is an operand in m0, so the compiler knows what that register holds.
 constexpr uint32_t kOutside = 0x80000000u;
 __device__ __forceinline__ void loadToLds(uint32_t ldsAt, uint32_t voff, __amdgpu_buffer_rsrc_t rsrc, uint32_t soff) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(ldsAt), "v"(voff), "s"(rsrc), "s"(soff));
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"{m0}"(ldsAt), "v"(voff), "s"(rsrc), "s"(soff));
 }
 // `left` = loads of this wavefront that may still be on their way.
 template <int left>
@@ -740,7 +741,7 @@ struct DirectScales {
   }
   __device__ __forceinline__ void issue(uint32_t lds, uint32_t wave, bool there) {
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)at, 0, 0x7fffffff, 0x00020000);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds + wave * 256),
+    asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"{m0}"(lds + wave * 256),
                  "v"(there ? voff : kOutside), "s"(rsrc));
     at += 4;
   }
@@ -844,7 +845,7 @@ __global__ void __launch_bounds__(WN *WM * 64, (kToSimd<T, WN * WM * 64, (SN * B
     if constexpr (TOUCH) {                    // sn.at is a slab further already, and sm.at too
       const uint64_t from = (wave == 0 ? sn.at : sm.at) + (kTouchAhead - 1) * 128;
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(uintptr_t)from, 0, 0x7fffffff, 0x00020000);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds0 + kLds),
+      asm volatile("s_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"{m0}"(lds0 + kLds),
                    "v"(leftN > kTouchAhead * P::kSlab ? touched : kOutside), "s"(rsrc));
     }
     nextOf(sn, leftN, todoN);

@@ -193,6 +193,22 @@ int main(void) {
     subprocess.run([str(exe)], check=True)
 
 
+def test_assembly_names_the_registers_it_uses():
+    """m0 holds the LDS address of a load into LDS: it is an operand of every such statement and is written by none, so that
+    the compiler never takes it to hold something else."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "flagcx_amd", "csrc")
+    loads = 0
+    for name in sorted(os.listdir(csrc)):
+        if name.endswith((".hip", ".hpp")):
+            for text in re.findall(r"asm volatile\((.*?)\);", open(os.path.join(csrc, name)).read(), re.S):
+                code, operands = text.split("::", 1) if "::" in text else (text, "")
+                assert not re.search(r"\bm0\b", code), (name, text)
+                if re.search(r"buffer_load\w* .*\blds\b", code):
+                    loads += 1
+                    assert '"{m0}"' in operands, (name, text)
+    assert loads >= 3
+
+
 def test_stride_blocks_match_the_header():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     text = re.sub(r"/\*.*?\*/", "", open(os.path.join(root, "include", "flagcx_amd", "fx_model.h")).read(), flags=re.S)
