@@ -119,6 +119,10 @@ __device__ __forceinline__ void panelOrder(uint32_t id, uint32_t mTiles, uint32_
 // eight columns at a time (4096 rows of 16 experts, 4096 x 4096: 202 -> 186 us, e4m3 144
 // -> 122; eight where there are more rounds: 300 -> 306 us for 8192 rows, e4m3 with 32
 // experts 222 -> 234).
+// Boundaries that do not ascend may count more tiles than the grid has, up to a whole
+// call's for every other expert: the counts end at kMostTiles, far above any grid's,
+// so that what they are multiplied with stays below 2^32.
+constexpr uint32_t kMostTiles = 1u << 26;
 template <int BN, int BM, bool ORDERED>
 __device__ __forceinline__ bool findTile(const ProductArgs &a, Tile *t) {
   uint32_t mt, nt, id = blockIdx.x;
@@ -138,8 +142,12 @@ __device__ __forceinline__ bool findTile(const ProductArgs &a, Tile *t) {
     rows = rowsOf(a, e + lane, &first);
     scan = waveScan(whole());
     tiles[0] += uniform((uint32_t)__shfl((int)scan, 63));
+    if (ORDERED && tiles[0] > kMostTiles) tiles[0] = kMostTiles;
 #pragma unroll
-    for (int k = 1; k < kKinds; k++) tiles[k] += (uint32_t)__popcll(__ballot(isKind(k)));
+    for (int k = 1; k < kKinds; k++) {
+      tiles[k] += (uint32_t)__popcll(__ballot(isKind(k)));
+      if (tiles[k] > kMostTiles) tiles[k] = kMostTiles;
+    }
   }
   uint32_t mTiles = 0;
 #pragma unroll

@@ -97,9 +97,10 @@ int fx_reduce_norm_grad(void *dx, void *dweight, const void *dy, const void *x,
  * `offsets` is a DEVICE array of experts + 1 ascending int32 values, read when
  * the call executes (routing need not reach the host); an expert may have no
  * rows.  Values outside [0, rows] are clamped and a descending pair is an empty
- * expert: nothing outside the buffers is ever touched.  Rows of y before
- * offsets[0] or from offsets[experts] on are left as they were.  offsets = NULL
- * with experts = 1: all rows, the plain product.
+ * expert: nothing outside the buffers is ever touched (rows that several experts
+ * claim then get one's results, or none).  Rows of y before offsets[0] or from
+ * offsets[experts] on are left as they were.  offsets = NULL with experts = 1: all
+ * rows, the plain product.
  * dtype (x, w): bf16 or fp16; out_dtype: dtype or fp32.  y overlaps nothing else.
  * Extents and experts < 2^31.  Calls that would need 2^32 threads in one launch are
  * not supported (9): 2^28 columns or more for few rows, 2^36 elements or more of y.

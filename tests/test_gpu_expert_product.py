@@ -628,3 +628,26 @@ def test_e4m3_sums_are_cut_as_documented(dev, out, kind, rows, n, k):
         assert (np.abs(cut - want) > np.abs(want) / 4).any()
     if kind == "below":
         assert (np.abs(cut - want) > 2.0 ** -11 * mag).all()
+
+
+def test_many_experts_that_claim_all_rows_touch_nothing_outside(dev):
+    """Boundaries 0, rows, 0, rows, ... of 131072 experts: their tiles, counted, are 2^30, and 2^32 in four columns of tiles.
+    All experts share one matrix, so a row is right or left alone."""
+    rows, n, k, experts = 1 << 20, 8, 8, 1 << 17
+    x, w = R.normal(N.DT_BF16, (rows, k), 1), R.normal(N.DT_BF16, (1, k, n), 2)
+    o = np.zeros(experts + 1, np.int32)
+    o[1::2] = rows
+    guard = np.full((256, n), 9, np.uint16)
+    with DevBufs(dev) as b:
+        dx, dw, do = b.put(x), b.put(w), b.put(o)
+        base = b.put(np.concatenate([guard, np.full((rows, n), 9, np.uint16), guard]))
+        st = dict(x=k, w=n, y=n, expert_w=0)
+        N.check(K.expert_product(base + guard.nbytes, dx, dw, do, experts, rows, n, k, N.DT_BF16, layout=K.W_KN, strides=st))
+        dev.sync()
+        y = dev.to_host(base, (rows + 512) * n, np.uint16).reshape(-1, n)
+    assert (y[:256] == 9).all() and (y[-256:] == 9).all()
+    y = y[256:-256]
+    done = ~(y == 9).all(axis=1)
+    want, mag = R.product(R.codes_to_f64(x, N.DT_BF16), R.codes_to_f64(w, N.DT_BF16), [0, rows], False)
+    bad = np.abs(R.codes_to_f64(y, N.DT_BF16) - want) > R.rounding(want, N.DT_BF16) * 1.01 + R.sum_bound(k, mag)
+    assert done.any() and not bad[done].any()
