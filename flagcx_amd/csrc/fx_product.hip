@@ -1,4 +1,4 @@
-// C entry points of the products grouped by expert: argument checks, then one launch.
+// C entry points of the products grouped by expert: argument checks, then the launch.
 #include "fx_product.hpp"
 
 using namespace fx;

@@ -1299,17 +1299,32 @@ flagcxResult_t launchProductBf16(const ProductArgs &a, int form, bool outF32, hi
 flagcxResult_t launchProductF16(const ProductArgs &a, int form, bool outF32, hipStream_t s);
 flagcxResult_t launchProductE4m3(const ProductArgs &a, int outDtype, hipStream_t s);
 
-inline flagcxResult_t launchGrid(const void *kernel, ProductArgs &a, uint32_t bn, uint32_t bm, bool dw, uint32_t threads, hipStream_t s) {
-  a.nTiles = (a.n + bn - 1) / bn;
+// A launch takes less than 2^32 threads: calls that need more (4096 experts with a row
+// each and 64,000 columns) go through their columns in several.  colBytes, outBytes:
+// from one column of the n side and of the output to the next; es: of an operand.
+inline flagcxResult_t launchGrid(const void *kernel, ProductArgs a, uint32_t bn, uint32_t bm, bool dw, uint32_t threads, size_t es,
+                                 size_t colBytes, size_t outBytes, hipStream_t s) {
   if (dw) a.mTiles = (a.m + bm - 1) / bm;
   else if (!a.offsets) a.mTiles = (a.rows + bm - 1) / bm;
   else a.mTiles = a.rows / bm + (a.experts < a.rows ? a.experts : a.rows);   // every expert's last tile may be partial
   const uint32_t reached = a.experts < a.rows ? a.experts : a.rows;
-  a.group = (uint64_t)a.nTiles * (a.rows / bm + reached / 2) <= 2 * kUnits ? 8 : 4;
-  const uint64_t grid = (uint64_t)a.nTiles * a.mTiles * (dw ? a.experts : 1);
-  if (grid * threads > 0xffffffffu) return flagcxNotSupported;   // the runtime's limit: 2^32 threads
-  void *argv[] = {&a};
-  return hipLaunchKernel(kernel, dim3((uint32_t)grid), dim3(threads), argv, 0, s) == hipSuccess ? flagcxSuccess : flagcxUnhandledDeviceError;
+  const uint64_t column = (uint64_t)a.mTiles * (dw ? a.experts : 1) * threads, most = 0xffffffffu / column;   // of tiles
+  const uint64_t unit = es == 1 && bn < FX_SCALE_GROUP ? FX_SCALE_GROUP : bn, columns = most * bn / unit * unit;
+  if (columns == 0 && (a.n + bn - 1) / bn > most) return flagcxNotSupported;
+  flagcxResult_t rc = flagcxSuccess;
+  for (uint64_t left = a.n; left && rc == flagcxSuccess;) {
+    a.n = (uint32_t)((left + bn - 1) / bn <= most ? left : columns);
+    a.nTiles = (a.n + bn - 1) / bn;
+    a.group = (uint64_t)a.nTiles * (a.rows / bm + reached / 2) <= 2 * kUnits ? 8 : 4;
+    void *argv[] = {&a};
+    if (hipLaunchKernel(kernel, dim3(a.nTiles * (uint32_t)(column / threads)), dim3(threads), argv, 0, s) != hipSuccess)
+      rc = flagcxUnhandledDeviceError;
+    left -= a.n;
+    a.pn = (const char *)a.pn + a.n * colBytes;
+    a.y = (char *)a.y + a.n * outBytes;
+    if (a.sn) a.sn += a.n / FX_SCALE_GROUP * a.ldsn;
+  }
+  return rc;
 }
 
 // SN = 1: any alignment; SN = 0: rows of less than a chunk
@@ -1319,7 +1334,8 @@ flagcxResult_t launchTiles(ProductArgs a, hipStream_t s) {
   if constexpr (SN == 1) kernel = reinterpret_cast<const void *>(productNear<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
   else if constexpr (SN != 0) kernel = reinterpret_cast<const void *>(productDirect<T, Out, BN, BM, WN, WM, SN, SM, NACROSS, MACROSS, DW, TOUCH>);
   else kernel = reinterpret_cast<const void *>(productGuarded<T, Out, BN, BM, WN, WM, NACROSS, MACROSS, DW>);
-  return launchGrid(kernel, a, BN, BM, DW, WN * WM * 64, s);
+  const size_t es = kBytes<T>;
+  return launchGrid(kernel, a, BN, BM, DW, WN * WM * 64, es, (NACROSS ? 1 : a.ldn) * es, sizeof(Out), s);
 }
 
 template <class T, class Out, int RN, int FM, int NW, int U>
@@ -1328,7 +1344,7 @@ flagcxResult_t launchThin(ProductArgs a, hipStream_t s) {
   const bool odd = ((uintptr_t)a.pn | (uintptr_t)a.pm | a.ldn * es | a.ldm * es | a.expertN * es) & 3;
   const void *kernel = odd ? reinterpret_cast<const void *>(productThin<T, Out, RN, FM, NW, U, true>)
                            : reinterpret_cast<const void *>(productThin<T, Out, RN, FM, NW, U, false>);
-  return launchGrid(kernel, a, 16 * RN, 16 * FM, false, NW * 64, s);
+  return launchGrid(kernel, a, 16 * RN, 16 * FM, false, NW * 64, es, a.ldn * es, sizeof(Out), s);
 }
 
 // Whole 16-byte chunks everywhere: what the direct kernels assume.  `inner` is the

@@ -102,8 +102,10 @@ int fx_reduce_norm_grad(void *dx, void *dweight, const void *dy, const void *x,
  * offsets[experts] on are left as they were.  offsets = NULL with experts = 1: all
  * rows, the plain product.
  * dtype (x, w): bf16 or fp16; out_dtype: dtype or fp32.  y overlaps nothing else.
- * Extents and experts < 2^31.  Calls that would need 2^32 threads in one launch are
- * not supported (9): 2^28 columns or more for few rows, 2^36 elements or more of y.
+ * Extents and experts < 2^31.  A launch takes less than 2^32 threads; calls with more
+ * columns than that go through them in several.  Where the rows of up to 256 columns
+ * need as many by themselves, the call is not supported (9): that takes four million
+ * experts with rows of their own, for dw eight million experts or 2^31 rows of dw.
  */
 enum { FX_WEIGHT_NK = 0, FX_WEIGHT_KN = 1 };
 typedef struct fxProductStrides {

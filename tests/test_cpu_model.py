@@ -102,6 +102,13 @@ def test_product_refusals():
     assert product(rows=0, y=None, x=None) == OK and product(n=0, y=None) == OK and product(experts=0, y=None) == OK
 
 
+def test_products_of_millions_of_experts_are_refused():
+    """Row tiles that need 2^32 threads by themselves: 512, 512 and four times 256 threads an expert."""
+    assert product(experts=1 << 24, rows=1 << 24) == NOT
+    assert K.expert_product_dw(P, P, P, P, 1 << 24, 64, 128, 256, N.DT_BF16) == NOT
+    assert K.expert_product_e4m3(P, P, P, P, P, P, 1 << 23, 1 << 23, 128, 300, N.DT_BF16) == NOT
+
+
 def test_product_dw_refusals():
     def dw(**kw):
         a = dict(dw=P, dy=P, x=P, offsets=P, experts=4, rows=64, n=128, k=256, dtype=N.DT_FP16)

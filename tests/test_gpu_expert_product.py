@@ -651,3 +651,49 @@ def test_many_experts_that_claim_all_rows_touch_nothing_outside(dev):
     want, mag = R.product(R.codes_to_f64(x, N.DT_BF16), R.codes_to_f64(w, N.DT_BF16), [0, rows], False)
     bad = np.abs(R.codes_to_f64(y, N.DT_BF16) - want) > R.rounding(want, N.DT_BF16) * 1.01 + R.sum_bound(k, mag)
     assert done.any() and not bad[done].any()
+
+
+def test_more_columns_than_one_launch_takes(dev):
+    """4096 experts with a row each share one matrix of so many columns that the call goes through them in two launches;
+    likewise the weights' gradient of a million experts, most of them without rows."""
+    experts, k = 4096, 16
+    x, o = R.normal(N.DT_BF16, (experts, k), 1), np.arange(experts + 1, dtype=np.int32)
+    for n, fp8 in ((62500, False), (123500, True)):
+        some = np.unique(np.concatenate([np.arange(0, n, 97), np.arange(61300, 61900), np.arange(n - 600, n)]))
+        kw = dict(x=k, w=k, y=n, expert_w=0)
+        with DevBufs(dev) as b:
+            dy, do = b.alloc(experts * n * 2), b.put(o)
+            if fp8:
+                rng = np.random.default_rng(2)
+                x8, w = (R.to_e4m3(np.clip(rng.standard_normal(s) * 120, -448, 448)) for s in ((experts, k), (n, k)))
+                xs, ws = np.exp2(rng.uniform(-9, 1, (experts, 1))).astype(np.float32), np.exp2(rng.uniform(-12, -4, (-(-n // 128), 1))).astype(np.float32)
+                st = dict(kw, xscale=1, wscale=1, expert_wscale=0)
+                N.check(K.expert_product_e4m3(dy, b.put(x8), b.put(xs), b.put(w), b.put(ws), do, experts, experts, n, k, N.DT_BF16, strides=st))
+                fx, fw = R.E4M3[x8] * xs, (R.E4M3[w] * np.repeat(ws.astype(np.float64), 128, axis=0)[:n])[some]
+            else:
+                w = R.normal(N.DT_BF16, (n, k), 2)
+                N.check(K.expert_product(dy, b.put(x), b.put(w), do, experts, experts, n, k, N.DT_BF16, strides=kw))
+                fx, fw = R.codes_to_f64(x, N.DT_BF16), R.codes_to_f64(w[some], N.DT_BF16)
+            dev.sync()
+            y = dev.to_host(dy, experts * n, np.uint16).reshape(experts, n)[:, some]
+        want, mag = fx @ fw.T, np.abs(fx) @ np.abs(fw).T
+        assert (np.abs(R.codes_to_f64(y, N.DT_BF16) - want) <= R.rounding(want, N.DT_BF16) * 1.01 + R.sum_bound(k + 8, mag)).all(), fp8
+    experts, rows, k = 1 << 20, 300, 2000                    # one column of dy: 2000 dw values an expert
+    dy, x = R.normal(N.DT_BF16, (rows, 1), 3), R.normal(N.DT_BF16, (rows, k), 4)
+    at = np.sort(np.random.default_rng(5).choice(experts, rows // 2, replace=False))         # the experts of two rows each
+    o = np.zeros(experts + 1, np.int32)
+    o[at + 1] = 2
+    o = np.cumsum(o).astype(np.int32)
+    f = lambda a: R.codes_to_f64(a, N.DT_BF16)  # noqa: E731
+    with DevBufs(dev) as b:
+        dw = b.alloc(experts * k * 2)
+        N.check(K.expert_product_dw(dw, b.put(dy), b.put(x), b.put(o), experts, rows, 1, k, N.DT_BF16))
+        dev.sync()
+        for i, e in enumerate(at):
+            got = f(dev.to_host(dw + int(e) * k * 2, k, np.uint16))
+            a, d = f(x[2 * i:2 * i + 2]), f(dy[2 * i:2 * i + 2])
+            want, mag = (d * a).sum(axis=0), np.abs(d * a).sum(axis=0)
+            assert (np.abs(got - want) <= R.rounding(want, N.DT_BF16) * 1.01 + R.sum_bound(2, mag)).all(), e
+        for e in (0, 1, 77777, experts - 1):
+            if e not in at:
+                assert not dev.to_host(dw + e * k * 2, k, np.uint16).any()
