@@ -697,3 +697,20 @@ def test_more_columns_than_one_launch_takes(dev):
         for e in (0, 1, 77777, experts - 1):
             if e not in at:
                 assert not dev.to_host(dw + e * k * 2, k, np.uint16).any()
+
+
+@pytest.mark.parametrize("out", [N.DT_BF16, N.DT_FP32])
+@pytest.mark.parametrize("rows,n,k,offsets", [(330, 208, 8320, [0, 90, 200, 330]), (330, 208, 16400, [0, 90, 200, 330]), (130, 1040, 8336, None),
+                                              (1600, 1040, 8320, [0, 520, 1090, 1600]), (1600, 1040, 16400, [0, 520, 1090, 1600]),
+                                              (4400, 1040, 8336, [0, 2150, 4400]), (300, 200, 8325, [0, 100, 300]),
+                                              (40, 200, 16400, [0, 10, 25, 40]), (12, 200, 8325, [0, 5, 12])])
+def test_e4m3_reductions_of_many_blocks(dev, out, rows, n, k, offsets):
+    """More than 64 groups of 128 (a wavefront holds 64 blocks' scales at a time), walked from another slab for each expert
+    and around the end, with a partial last group."""
+    print(out, rows, n, k, flush=True)
+    run8(dev, rows, n, k, None if offsets is None else np.array(offsets, np.int32), out, seed=k)
+
+
+@pytest.mark.parametrize("rows,n,k,offsets", [(2600, 4160, 8336, [0, 1200, 2600]), (4400, 2080, 8336, [0, 2150, 4400])])
+def test_e4m3_reductions_of_many_blocks_in_the_largest_tiles(dev, rows, n, k, offsets):
+    run8(dev, rows, n, k, np.array(offsets, np.int32), N.DT_BF16, seed=k)

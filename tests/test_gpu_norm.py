@@ -351,3 +351,34 @@ def test_norm_gradients_in_the_workspace_of_a_larger_call(dev, rows, most, cols,
     f = lambda a: R.codes_to_f64(a, t)  # noqa: E731
     edx, edw, bx, bw = R.norm_grad(f(dy), f(x), f(w), None, EPS)
     assert (np.abs(gx - edx) <= R.rounding(edx, t) * 1.01 + bx).all() and (np.abs(gw - edw) <= R.rounding(edw, t) * 1.01 + bw).all()
+
+
+# Rows enough for results of more than 32 MiB (streamed), in each way that a row is held: one or two octets to a lane of a
+# wavefront, two or four to a lane of a workgroup.
+@pytest.mark.parametrize("name,rows,cols", [("bf16", 23000, 500), ("fp16", 12000, 1000), ("bf16", 2900, 4003), ("bf16", 1400, 8192),
+                                            ("fp16", 700, 16500), ("fp32", 450, 16000), ("fp32", 300, 32001)])
+def test_norm_of_large_calls(dev, name, rows, cols):
+    print(name, rows, cols, flush=True)
+    t = TYPES[name]
+    assert rows * cols * (N.DTYPE_SIZE[t] + 1) > 32 << 20
+    run_norm(dev, t, rows, cols, 2, quant=True, seed=cols)
+    run_norm(dev, t, rows, cols, 1, seed=cols, alias="total=residual")
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("cols", [5003, 8192, 8200, 16384])
+def test_norm_gradients_of_several_rows_a_workgroup(dev, name, cols):
+    """Wide rows, more of them than workgroups: the next row loaded ahead or not, the sums of two rows in turn."""
+    print(name, cols, flush=True)
+    run_grad(dev, TYPES[name], 600, cols, seed=cols)
+
+
+# More than 128 MiB read and written (streamed), in each way that a row is held.
+@pytest.mark.parametrize("name,rows,cols,alias", [("bf16", 34000, 500, None), ("fp16", 17500, 1000, "dy"), ("bf16", 4200, 4096, "dtotal"),
+                                                  ("bf16", 2200, 8000, "dy"), ("fp16", 1100, 16000, "dtotal"), ("fp32", 530, 16384, "dy"),
+                                                  ("fp32", 4300, 2001, None)])
+def test_norm_gradients_of_large_calls(dev, name, rows, cols, alias):
+    print(name, rows, cols, alias, flush=True)
+    t = TYPES[name]
+    assert rows * cols * N.DTYPE_SIZE[t] * 4 > 128 << 20
+    run_grad(dev, t, rows, cols, alias=alias, seed=cols)
