@@ -7,8 +7,11 @@
 // the threads, and the results leave from the same registers.  The arithmetic is a
 // few operations per element; HBM bounds it.  Rows of up to 64 V octets are a
 // wavefront's, four to a workgroup; longer ones a workgroup's, with as many
-// wavefronts as they need; rows longer than the registers hold are read twice.
-// Measured: 16384 x 8192, two bf16 inputs and the residual to e4m3, 214 us (5.65 TB/s of
+// wavefronts as they need; rows longer than the registers hold are read twice.  fp32
+// rows of more than 16384 columns (gradients: 8192) do not quite fit: up to 116 bytes a
+// lane go to scratch memory (gradients of 4096 x 16384: fp32 275 us, 3.9 TB/s; bf16 109,
+// 4.9 TB/s).
+// Measured: 16384 x 8192, two bf16 inputs and the residual to e4m3, 215 us (5.6 TB/s of
 // exactly the operands' bytes); gradients of 8192 x 4096 bf16 47 us (5.7 TB/s); one row of
 // 8192 with eight inputs 6 us, a launch being 4.
 #include "flagcx_amd/fx_kernels.h"
